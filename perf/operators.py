@@ -224,25 +224,29 @@ def _plain_append(s, eps):
 def _plain_attend(s):
     c, case = s["cache"], s["case"]
     h, hkv, d, page = case["heads"], case["kv_heads"], case["dim"], case["page"]
-    out = torch.empty_like(s["q"])
-    at = 0
-    for b, (past, new) in enumerate(c.sizes):
-        n = past + new
-        pages = c.table[b, :-(-n // page)].long()
-        k = c.k[pages].reshape(-1, hkv, d)[:n].float()
-        v = c.v[pages].reshape(-1, hkv, d)[:n].float()
-        q = s["q"][at:at + new].float().reshape(new, hkv, h // hkv, d)
-        scores = torch.einsum("tgrd,sgd->grts", q, k) * (1.0 / math.sqrt(d))
-        if new > 1:
-            later = torch.arange(n, device=k.device)[None] > past + torch.arange(new, device=k.device)[:, None]
-            scores.masked_fill_(later, -math.inf)
+    new, keys, n = c.most_new, max(p + n for p, n in c.sizes), len(c.sizes)
+    # all sequences at once, padded to the longest, as far as 2 GB of scores (and of keys in 32 bits) go
+    some = max(1, min(n, 2 ** 29 // (keys * max(h * new, hkv * d))))
+    place, key = torch.arange(new, device=c.k.device), torch.arange(keys, device=c.k.device)
+    out = []
+    for b in range(0, n, some):
+        first, count, past = c.offsets[b:b + some + 1].long(), c.offsets[b:b + some + 1].diff().long(), c.lengths[b:b + some].long()
+        rows = (first[:-1, None] + place).clamp_max(c.tokens - 1)
+        q = s["q"][rows].float().reshape(-1, new, hkv, h // hkv, d)
+        pages = c.table[b:b + some, :-(-keys // page)].long().clamp_min(0)
+        k = c.k[pages].reshape(len(past), -1, hkv, d)[:, :keys].float()
+        v = c.v[pages].reshape(len(past), -1, hkv, d)[:, :keys].float()
+        scores = torch.einsum("btgrd,bsgd->bgrts", q, k) * (1.0 / math.sqrt(d))
+        scores.masked_fill_((key > past[:, None, None] + place[:, None])[:, None, None], -math.inf)
         scores -= scores.amax(-1, keepdim=True)
         scores.exp_()
         total = scores.sum(-1)
-        o = torch.einsum("grts,sgd->tgrd", scores, v) / total.permute(2, 0, 1)[..., None]
-        out[at:at + new] = o.reshape(new, h, d)
-        at += new
-    return out
+        o = torch.einsum("bgrts,bsgd->btgrd", scores, v) / total.permute(0, 3, 1, 2)[..., None]
+        tokens = sum(m for _, m in c.sizes[b:b + some])
+        seq = torch.repeat_interleave(torch.arange(len(past), device=first.device), count, output_size=tokens)
+        i = torch.arange(tokens, device=first.device) - (first[:-1] - first[0])[seq]
+        out.append(o[seq, i].reshape(tokens, h, d).bfloat16())
+    return torch.cat(out)
 
 
 def _plain_verify(s):
