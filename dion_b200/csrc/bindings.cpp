@@ -1292,6 +1292,160 @@ void symm_reduce_scatter(const Tensor& inp, Tensor out, at::IntArrayRef peers, i
       at::cuda::getCurrentCUDAStream()));
 }
 
+
+// ----------------------------------------------------------------------------- paged cache
+
+// Pages [pages, page_size, kv heads, head_dim] in any order that TMA and 16-byte accesses can take, with the table, offsets
+// and lengths of the sequences whose new tokens the rows of q are.  Sets what the two structs name alike.
+template <typename Args>
+void describe_paged(Args& p, const char* name, const Tensor& q, const Tensor& k_pages, const Tensor& v_pages,
+                    const Tensor& page_table, const Tensor& offsets, const Tensor& lengths, const Tensor& status) {
+  TORCH_CHECK_VALUE(q.dim() == 3, name, ": queries are [tokens, heads, head_dim], not ", q.sizes());
+  TORCH_CHECK_VALUE(k_pages.dim() == 4 && v_pages.sizes() == k_pages.sizes(), name,
+                    ": key and value pages are [pages, page_size, kv heads, head_dim], both of one shape, not ", k_pages.sizes(), " and ",
+                    v_pages.sizes());
+  const int64_t size = k_pages.size(1), heads = q.size(1), kv_heads = k_pages.size(2), dim = q.size(2);
+  TORCH_CHECK_VALUE(size >= 16 && (size & (size - 1)) == 0 && size <= (1 << 30), name,
+                    ": the size of a page is a power of two from 16 on, not ", size);
+  TORCH_CHECK_VALUE(dim == k_pages.size(3) && heads > 0 && kv_heads > 0 && heads % kv_heads == 0, name, ": ", heads, " query heads of ",
+                    dim, " do not go with ", kv_heads, " cached heads of ", k_pages.size(3));
+  for (const Tensor* t : {&k_pages, &v_pages}) {
+    TORCH_CHECK_VALUE(t->scalar_type() == q.scalar_type() && t->device() == q.device(), name,
+                      ": tensors of one type on one device, not ", t->scalar_type(), " on ", t->device(), " beside ", q.scalar_type(), " on ",
+                      q.device());
+    bool fits = on_16_bytes(*t) && t->stride(3) == 1;
+    for (int i = 0; i < 3; ++i) fits = fits && (t->size(i) == 1 || (t->stride(i) > 0 && t->stride(i) % 8 == 0));
+    TORCH_CHECK_VALUE(fits, name, ": pages start on 16 bytes, with the head dimension contiguous and the other strides positive multiples of 8, not ",
+                      t->strides());
+  }
+  const int64_t seqs = lengths.dim() == 1 ? lengths.size(0) : -1;
+  for (const Tensor* t : {&page_table, &offsets, &lengths})
+    TORCH_CHECK_VALUE(t->scalar_type() == at::kInt && t->device() == q.device() && t->dim() == (t == &page_table ? 2 : 1) &&
+                          (t->size(-1) <= 1 || t->stride(-1) == 1),
+                      name, ": page table, offsets and lengths are int32, on the device of the queries, with contiguous rows");
+  TORCH_CHECK_VALUE(page_table.size(0) == seqs && offsets.size(0) == seqs + 1, name, ": ", seqs,
+                    " lengths need as many rows of the page table and ", seqs + 1, " offsets");
+  TORCH_CHECK(status.scalar_type() == at::kInt && status.device() == q.device(), name, ": status is int32 on the same device");
+  const int64_t most = std::numeric_limits<int>::max();
+  TORCH_CHECK_VALUE(q.size(0) <= most && heads * dim <= most && k_pages.size(0) <= most && page_table.size(1) <= most && seqs < most, name,
+                    ": more than 2^31 - 1 tokens, pages or sequences");
+  p.page_table = page_table.data_ptr<int>();
+  p.offsets = offsets.data_ptr<int>();
+  p.lengths = lengths.data_ptr<int>();
+  p.status = status.data_ptr<int>();
+  p.table_pitch = page_table.stride(0);
+  p.tokens = (int)q.size(0);
+  p.seqs = (int)seqs;
+  p.heads = (int)heads;
+  p.kv_heads = (int)kv_heads;
+  p.page_shift = __builtin_ctzll((unsigned long long)size);
+  p.pages = (int)k_pages.size(0);
+  p.max_pages = (int)page_table.size(1);
+  p.k_page = k_pages.stride(0), p.k_row = k_pages.stride(1), p.k_head = k_pages.stride(2);
+  p.v_page = v_pages.stride(0), p.v_row = v_pages.stride(1), p.v_head = v_pages.stride(2);
+}
+
+const __nv_bfloat16* bf16_data(const Tensor& t) { return reinterpret_cast<const __nv_bfloat16*>(t.data_ptr()); }
+__nv_bfloat16* bf16_data_out(const Tensor& t) { return reinterpret_cast<__nv_bfloat16*>(t.data_ptr()); }
+
+// [tokens, heads, head_dim] with 16-byte rows; others are copied
+Tensor with_rows(const Tensor& t) {
+  const bool fits = on_16_bytes(t) && t.stride(2) == 1 && (t.size(0) == 1 || t.stride(0) % 8 == 0) &&
+                    (t.size(1) == 1 || t.stride(1) % 8 == 0);
+  return fits ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
+Tensor paged_append(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& cos_, const Tensor& sin_, Tensor k_pages,
+                    Tensor v_pages, const Tensor& page_table, const Tensor& offsets, const Tensor& lengths, double eps,
+                    Tensor status) {
+  dion::PagedAppend p;
+  const c10::cuda::CUDAGuard guard(q_.device());
+  describe_paged(p, "paged_append", q_, k_pages, v_pages, page_table, offsets, lengths, status);
+  const int64_t N = q_.size(0), D = q_.size(2);
+  for (const Tensor* t : {&k_, &v_})
+    TORCH_CHECK_VALUE(t->dim() == 3 && t->size(0) == N && t->size(1) == p.kv_heads && t->size(2) == D && t->scalar_type() == q_.scalar_type() &&
+                          t->device() == q_.device(),
+                      "paged_append: keys and values are [", N, ", ", p.kv_heads, ", ", D, "], of the type and device of the queries, not ", t->sizes());
+  for (const Tensor* t : {&cos_, &sin_})
+    TORCH_CHECK_VALUE(t->dim() == 2 && t->size(1) == D / 2 && t->sizes() == cos_.sizes() && t->scalar_type() == cos_.scalar_type() &&
+                          (t->scalar_type() == at::kBFloat16 || t->scalar_type() == at::kFloat) && t->device() == q_.device(),
+                      "paged_append: cos and sin are two tables [positions, ", D / 2, "] of one type, bf16 or fp32, on the device of the queries");
+  if (N == 0 || p.seqs == 0) return at::zeros({N, p.heads, D}, q_.options());
+  auto table = [](const Tensor& t) {
+    return on_16_bytes(t) && t.stride(1) == 1 && t.stride(0) * t.element_size() % 16 == 0 ? t : t.clone(at::MemoryFormat::Contiguous);
+  };
+  const Tensor q = with_rows(q_), k = with_rows(k_), v = with_rows(v_), cos = table(cos_), sin = table(sin_);
+  Tensor out = at::empty({N, p.heads, D}, q.options());
+  p.q = bf16_data(q), p.k = bf16_data(k), p.v = bf16_data(v);
+  p.q_out = bf16_data_out(out), p.k_pages = bf16_data_out(k_pages), p.v_pages = bf16_data_out(v_pages);
+  p.cos = cos.data_ptr(), p.sin = sin.data_ptr();
+  p.q_token = q.stride(0), p.q_head = q.stride(1);
+  p.k_token = k.stride(0), p.k_in_head = k.stride(1);
+  p.v_token = v.stride(0), p.v_in_head = v.stride(1);
+  p.cos_row = cos.stride(0), p.sin_row = sin.stride(0), p.table_rows = cos.size(0);
+  p.eps = (float)eps;
+  DION_CUDA_CHECK(dion::paged_append_launch(p, (int)D, cos.scalar_type() == at::kFloat, at::cuda::getCurrentCUDAStream()));
+  return out;
+}
+
+Tensor paged_attention(const Tensor& q_, const Tensor& k_pages, const Tensor& v_pages, const Tensor& page_table,
+                       const Tensor& offsets, const Tensor& lengths, double scale, int64_t max_new, Tensor status) {
+  dion::PagedAttention p;
+  const c10::cuda::CUDAGuard guard(q_.device());
+  describe_paged(p, "paged_attention", q_, k_pages, v_pages, page_table, offsets, lengths, status);
+  const int64_t N = q_.size(0), D = q_.size(2);
+  if (N == 0 || p.seqs == 0) return at::zeros({N, p.heads, D}, q_.options());
+  const Tensor q = with_rows(q_);
+  Tensor out = at::empty({N, p.heads, D}, q.options());
+  p.q = bf16_data(q), p.k_pages = bf16_data(k_pages), p.v_pages = bf16_data(v_pages);
+  p.out = bf16_data_out(out);
+  p.q_token = q.stride(0), p.q_head = q.stride(1);
+  p.max_new = (int)std::min(max_new, N);
+  p.scale = (float)scale;
+  DION_CUDA_CHECK(dion::paged_attention_launch(p, (int)D, at::cuda::getCurrentCUDAStream()));
+  return out;
+}
+
+std::tuple<Tensor, Tensor> verify_drafts(const Tensor& target, const std::optional<Tensor>& draft, const Tensor& tokens,
+                                         const Tensor& uniforms, Tensor status) {
+  const c10::cuda::CUDAGuard guard(target.device());
+  TORCH_CHECK_VALUE(target.dim() == 3 && target.size(1) >= 1 && target.size(2) >= 1 && target.scalar_type() == at::kFloat,
+                    "verify_drafts: the target's probabilities are fp32 [sequences, drafts + 1, vocabulary], not ", target.scalar_type(), " ", target.sizes());
+  const int64_t B = target.size(0), K = target.size(1) - 1, V = target.size(2);
+  TORCH_CHECK_VALUE(tokens.dim() == 2 && tokens.size(0) == B && tokens.size(1) == K && tokens.scalar_type() == at::kLong,
+                    "verify_drafts: drafted tokens are int64 [", B, ", ", K, "]");
+  TORCH_CHECK_VALUE(!draft.has_value() || (draft->dim() == 3 && draft->size(0) == B && draft->size(1) == K && draft->size(2) == V &&
+                                           draft->scalar_type() == at::kFloat),
+                    "verify_drafts: the draft's probabilities are fp32 [", B, ", ", K, ", ", V, "]");
+  TORCH_CHECK_VALUE(uniforms.dim() == 2 && uniforms.size(0) == B && uniforms.size(1) == K + 1 && uniforms.scalar_type() == at::kFloat,
+                    "verify_drafts: uniforms are fp32 [", B, ", ", K + 1, "]");
+  TORCH_CHECK_VALUE(tokens.device() == target.device() && uniforms.device() == target.device() &&
+                        (!draft.has_value() || draft->device() == target.device()) && status.device() == target.device(),
+                    "verify_drafts: tensors on one device");
+  TORCH_CHECK_VALUE(V <= std::numeric_limits<int>::max() && B <= std::numeric_limits<int>::max() && K < std::numeric_limits<int>::max(),
+                    "verify_drafts: more than 2^31 - 1 sequences, drafts or tokens of the vocabulary");
+  Tensor accepted = at::empty({B}, tokens.options()), token = at::empty({B}, tokens.options());
+  if (B == 0) return {accepted, token};
+  auto rows = [](const Tensor& t) { return t.stride(-1) == 1 || t.size(-1) <= 1 ? t : t.contiguous(); };
+  const Tensor t = rows(target), x = rows(tokens), u = rows(uniforms);
+  Tensor d;
+  dion::VerifyDrafts p{};
+  if (draft.has_value()) {
+    d = rows(*draft);
+    p.draft = d.data_ptr<float>();
+    p.draft_seq = d.stride(0), p.draft_row = d.stride(1);
+  }
+  p.target = t.data_ptr<float>(), p.uniforms = u.data_ptr<float>();
+  p.tokens = reinterpret_cast<const long long*>(x.data_ptr<int64_t>());
+  p.accepted = reinterpret_cast<long long*>(accepted.data_ptr<int64_t>());
+  p.token = reinterpret_cast<long long*>(token.data_ptr<int64_t>());
+  p.status = status.data_ptr<int>();
+  p.target_seq = t.stride(0), p.target_row = t.stride(1), p.uniforms_seq = u.stride(0), p.tokens_seq = x.stride(0);
+  p.seqs = (int)B, p.drafts = (int)K, p.vocab = (int)V;
+  DION_CUDA_CHECK(dion::verify_drafts_launch(p, at::cuda::getCurrentCUDAStream()));
+  return {accepted, token};
+}
+
 }  // namespace
 
 TORCH_LIBRARY(dion_b200, m) {
@@ -1383,6 +1537,14 @@ TORCH_LIBRARY(dion_b200, m) {
       "Tensor(d!)? ss, bool finish, float eps, Tensor(e!)? Qn, Tensor(f!)? Qs, int qs_col0, int[] peers, int flag_off, "
       "int channel, int rank, int epoch, int budget_ns, Tensor(g!) status) -> ()");
   m.def("dion_q_norm(Tensor R32, Tensor ss, Tensor Qm, float eps, Tensor(a!)? Qn, Tensor(b!)? Qs, int qs_col0) -> ()");
+  m.def(
+      "paged_append(Tensor q, Tensor k, Tensor v, Tensor cos, Tensor sin, Tensor(a!) k_pages, Tensor(b!) v_pages, "
+      "Tensor page_table, Tensor new_offsets, Tensor lengths, float eps, Tensor(c!) status) -> Tensor");
+  m.def(
+      "paged_attention(Tensor q, Tensor k_pages, Tensor v_pages, Tensor page_table, Tensor new_offsets, Tensor lengths, "
+      "float scale, int max_new, Tensor(a!) status) -> Tensor");
+  m.def(
+      "verify_drafts(Tensor target, Tensor? draft, Tensor tokens, Tensor uniforms, Tensor(a!) status) -> (Tensor, Tensor)");
   m.def("launch_count() -> int", &launch_count);
   m.def(
       "gemm_plan(Tensor a, Tensor b, Tensor? c, Tensor d, float beta=0, int act=0, bool symmetric=False, int block_n=0, int pair=0, "
@@ -1421,6 +1583,9 @@ TORCH_LIBRARY_IMPL(dion_b200, CUDA, m) {
   m.impl("gram_many", &gram_many);
   m.impl("attn_fwd", &attn_fwd);
   m.impl("attn_bwd", &attn_bwd);
+  m.impl("paged_append", &paged_append);
+  m.impl("paged_attention", &paged_attention);
+  m.impl("verify_drafts", &verify_drafts);
   m.impl("refine_prep", &refine_prep);
   m.impl("slot_reduce", &slot_reduce);
   m.impl("slot_reduce_bf16", &slot_reduce_bf16);

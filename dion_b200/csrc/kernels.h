@@ -1,6 +1,7 @@
 // Host launchers of the non-GEMM sm_100a kernels (plain CUDA types only).
 #pragma once
 
+#include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -298,5 +299,45 @@ struct QNormArgs {
   int qs_col0, qs_cols;
 };
 cudaError_t q_norm_launch(const QNormArgs& a, cudaStream_t s);
+
+// ---------------------------------------------------------------------------
+// The paged cache of keys and values (paged_append.cu, paged_attention.cu)
+// ---------------------------------------------------------------------------
+// Strides are in elements, the head dimension is contiguous everywhere; rows start on 16 bytes.
+struct PagedAppend {
+  const __nv_bfloat16 *q, *k, *v;
+  __nv_bfloat16 *q_out, *k_pages, *v_pages;  // q_out [tokens, heads, head_dim]
+  const void *cos, *sin;                     // [table_rows, head_dim / 2], bf16 or fp32
+  const int *page_table, *offsets, *lengths;
+  int* status;
+  long long q_token, q_head, k_token, k_in_head, v_token, v_in_head;
+  long long k_page, k_row, k_head, v_page, v_row, v_head, cos_row, sin_row, table_pitch, table_rows;
+  int tokens, seqs, heads, kv_heads, page_shift, pages, max_pages;
+  int tokens_per_block;  // the launcher's
+  float eps;             // negative: no norm
+};
+cudaError_t paged_append_launch(PagedAppend p, int head_dim, bool wide_tables, cudaStream_t stream);
+
+struct PagedAttention {
+  const __nv_bfloat16 *q, *k_pages, *v_pages;
+  __nv_bfloat16* out;  // [tokens, heads, head_dim]
+  const int *page_table, *offsets, *lengths;
+  int* status;
+  long long q_token, q_head, k_page, k_row, k_head, v_page, v_row, v_head, table_pitch;
+  int tokens, seqs, heads, kv_heads, page_shift, pages, max_pages, max_new;
+  float scale;
+};
+cudaError_t paged_attention_launch(const PagedAttention& p, int head_dim, cudaStream_t stream);
+
+// Drafted tokens against the target's probabilities (verify.cu); rows of `vocab` contiguous floats
+struct VerifyDrafts {
+  const float *target, *draft, *uniforms;  // draft null: the drafts were certain
+  const long long* tokens;
+  long long *accepted, *token;
+  int* status;
+  long long target_seq, target_row, draft_seq, draft_row, uniforms_seq, tokens_seq;
+  int seqs, drafts, vocab;
+};
+cudaError_t verify_drafts_launch(const VerifyDrafts& p, cudaStream_t stream);
 
 }  // namespace dion

@@ -15,4 +15,5 @@ from .multi_tensor import (  # noqa: F401
     muon_apply,
     muon_momentum,
 )
+from .paged import paged_append, paged_attention, verify_drafts  # noqa: F401
 from .runtime import DionKernelError, check_status, launch_count  # noqa: F401
