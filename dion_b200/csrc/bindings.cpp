@@ -1395,6 +1395,7 @@ Tensor paged_attention(const Tensor& q_, const Tensor& k_pages, const Tensor& v_
   describe_paged(p, "paged_attention", q_, k_pages, v_pages, page_table, offsets, lengths, status);
   const int64_t N = q_.size(0), D = q_.size(2);
   if (N == 0 || p.seqs == 0) return at::zeros({N, p.heads, D}, q_.options());
+  TORCH_CHECK_VALUE(p.pages > 0, "paged_attention: there are no pages");
   const Tensor q = with_rows(q_);
   Tensor out = at::empty({N, p.heads, D}, q.options());
   p.q = bf16_data(q), p.k_pages = bf16_data(k_pages), p.v_pages = bf16_data(v_pages);
@@ -1402,7 +1403,10 @@ Tensor paged_attention(const Tensor& q_, const Tensor& k_pages, const Tensor& v_
   p.q_token = q.stride(0), p.q_head = q.stride(1);
   p.max_new = (int)std::min(max_new, N);
   p.scale = (float)scale;
-  DION_CUDA_CHECK(dion::paged_attention_launch(p, (int)D, at::cuda::getCurrentCUDAStream()));
+  Tensor work = at::empty({dion::paged_attention_workspace(p, (int)D)}, q.options().dtype(at::kByte));
+  int launches = 1;
+  DION_CUDA_CHECK(dion::paged_attention_launch(p, (int)D, work.data_ptr(), &launches, at::cuda::getCurrentCUDAStream()));
+  g_launches.fetch_add(launches - 1, std::memory_order_relaxed);
   return out;
 }
 
