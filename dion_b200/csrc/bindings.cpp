@@ -1404,9 +1404,8 @@ Tensor paged_attention(const Tensor& q_, const Tensor& k_pages, const Tensor& v_
   p.max_new = (int)std::min(max_new, N);
   p.scale = (float)scale;
   Tensor work = at::empty({dion::paged_attention_workspace(p, (int)D)}, q.options().dtype(at::kByte));
-  int launches = 1;
-  DION_CUDA_CHECK(dion::paged_attention_launch(p, (int)D, work.data_ptr(), &launches, at::cuda::getCurrentCUDAStream()));
-  g_launches.fetch_add(launches - 1, std::memory_order_relaxed);
+  DION_CUDA_CHECK(dion::paged_attention_launch(p, (int)D, work.data_ptr(), at::cuda::getCurrentCUDAStream()));
+  g_launches.fetch_add(1, std::memory_order_relaxed);  // the parts are joined by a second one
   return out;
 }
 
@@ -1426,8 +1425,8 @@ std::tuple<Tensor, Tensor> verify_drafts(const Tensor& target, const std::option
   TORCH_CHECK_VALUE(tokens.device() == target.device() && uniforms.device() == target.device() &&
                         (!draft.has_value() || draft->device() == target.device()) && status.device() == target.device(),
                     "verify_drafts: tensors on one device");
-  TORCH_CHECK_VALUE(V <= std::numeric_limits<int>::max() && B <= std::numeric_limits<int>::max() && K < std::numeric_limits<int>::max(),
-                    "verify_drafts: more than 2^31 - 1 sequences, drafts or tokens of the vocabulary");
+  TORCH_CHECK_VALUE(V < (1ll << 31) - (1 << 16) && B < (1 << 28) && K < (1ll << 31) - 64,
+                    "verify_drafts: more sequences, drafts or tokens of the vocabulary than 32-bit indices take");
   Tensor accepted = at::empty({B}, tokens.options()), token = at::empty({B}, tokens.options());
   if (B == 0) return {accepted, token};
   auto rows = [](const Tensor& t) { return t.stride(-1) == 1 || t.size(-1) <= 1 ? t : t.contiguous(); };

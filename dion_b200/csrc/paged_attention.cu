@@ -26,9 +26,30 @@ typedef __nv_bfloat16 bf16;
 
 // ---------------------------------------------------------------------------------- the work and its shares
 
-// A sequence of the call: rows first .. first + n, keys = cached + new.  n = 0 where there is nothing to do or something is wrong.
+// What is worth a CTA.  One token over 1000 keys of 8 kv heads (us): 12.1 at 64, 12.9 at 128, 14.2 at 256; 6 heads of 777 keys 13.3,
+// 13.6 and 14.7
+constexpr int kShareCost = 64;
+
+// How rows are put together: `group` query heads of one kv head (`subs` such groups make all of its heads, where these are more than
+// a tile has rows) times `tokens` tokens are one tile of `height` rows, `tiles` of which go together.
+struct Tiling {
+  int height, tiles, group, subs, heads, tokens;  // heads: kv heads x subs; tokens: of all `tiles`
+  int fixed;                                      // what such rows cost apart from their keys, in keys
+  FastDiv by_group;
+  Tiling() = default;
+  Tiling(const PagedAttention& p, int height_, int tiles_, int fixed_) : height(height_), tiles(tiles_), fixed(fixed_) {
+    const int all = p.heads / p.kv_heads;
+    subs = (all + height - 1) / height;
+    group = (all + subs - 1) / subs;
+    heads = p.kv_heads * subs;
+    tokens = height / group * tiles;
+    by_group = FastDiv(group);
+  }
+};
+
+// A sequence of the call: rows first .. first + n, cached + n keys.  n = 0 where there is nothing to do or something is wrong.
 struct Sequence {
-  int first, n, keys;
+  int first, n, cached;
   bool bad;
 };
 __device__ __forceinline__ Sequence sequence(const PagedAttention& p, int b) {
@@ -37,15 +58,183 @@ __device__ __forceinline__ Sequence sequence(const PagedAttention& p, int b) {
   if (n == 0) return s;
   const long long most = min((long long)p.max_pages << p.page_shift, 0x7fffffffll - 1024);
   s.bad = first < 0 || n < 0 || end > p.tokens || cached < 0 || cached + n > most || n > p.max_new;
-  if (!s.bad) s = Sequence{(int)first, (int)n, (int)(cached + n), false};
+  if (!s.bad) s = Sequence{(int)first, (int)n, (int)cached, false};
   return s;
+}
+
+// An item is the rows of `tokens` tokens of one sequence and (part of a) kv head, with all keys that the last of them sees.  It costs
+// as much as its keys and `fixed` more.  Costs have a closed form, so that any position in the line of all items is found without
+// going through it.
+struct Costs {
+  int tokens, fixed, items;  // of a sequence, per head
+  Sequence s;
+  __device__ __forceinline__ Costs(const Sequence& s_, const Tiling& tl)
+      : tokens(tl.tokens), fixed(tl.fixed), items((int)(((long long)s_.n + tl.tokens - 1) / tl.tokens)), s(s_) {}
+  __device__ __forceinline__ int keys(int item) const { return (int)min((long long)s.cached + (item + 1ll) * tokens, (long long)s.cached + s.n); }
+  __device__ __forceinline__ long long before(int item) const { return item * ((long long)s.cached + fixed) + (long long)tokens * item * (item + 1ll) / 2; }
+  __device__ __forceinline__ long long head() const { return items > 0 ? before(items - 1) + fixed + s.cached + s.n : 0; }
+};
+
+// Goes through a CTA's share: item `item` of head `head` (of tiling.heads) of sequence b, units begin .. end of its `units` units
+// of K keys.  A share ends inside an item at a whole unit, or, where the item is small against the shares, at its nearer end.
+// Every warp has one in shared memory, which its first lane moves on: in registers it would cost the softmax loops theirs.
+template <int K>
+struct Walk {
+  long long to, at;  // positions in the line of all items: the share's end, this item's start
+  int share;         // a share's cost, as far as it is comparable to an item's
+  int b, head, item, begin, end, units, keys;
+  int first, n, cached;  // of the sequence
+  __device__ __forceinline__ bool valid() const { return at < to; }
+  // the unit at position y of this item's cost
+  __device__ __forceinline__ int cut(long long y, long long cost) const {
+    if (4 * cost <= share) return 2 * y < cost ? 0 : units;
+    return (int)(y * units / cost);
+  }
+  __device__ __forceinline__ void enter(const Tiling& tl, long long from) {
+    keys = Costs(Sequence{first, n, cached, false}, tl).keys(item);
+    units = (keys + K - 1) / K;
+    const long long cost = (long long)keys + tl.fixed;
+    begin = from <= at ? 0 : cut(from - at, cost);
+    end = to >= at + cost ? units : cut(to - at, cost);
+  }
+  __device__ __forceinline__ void take(const Sequence& s) { first = s.first, n = s.n, cached = s.cached; }
+  __device__ void next(const PagedAttention& p, const Tiling& tl) {
+    do {
+      at += (long long)keys + tl.fixed;
+      if (at >= to) return;
+      if ((++item) * (long long)tl.tokens >= n) {
+        item = 0;
+        if (++head == tl.heads) {
+          head = 0;
+          Sequence s;
+          do {
+            if (++b >= p.seqs) {
+              at = to;
+              return;
+            }
+            s = sequence(p, b);
+          } while (s.n == 0);
+          take(s);
+        }
+      }
+      enter(tl, at);
+    } while (begin >= end);
+  }
+  // by a whole warp
+  __device__ __forceinline__ void next(const PagedAttention& p, const Tiling& tl, int lane) {
+    __syncwarp();
+    if (lane == 0) next(p, tl);
+    __syncwarp();
+  }
+};
+
+template <int WARPS>
+struct ShareScratch {  // of the block, in shared memory
+  long long sums[WARPS], start;
+  int b;
+};
+
+// Finds this CTA's share with the whole block and gives it to every warp.
+template <int K, int WARPS>
+__device__ __forceinline__ void my_share(const PagedAttention& p, const Tiling& tl, ShareScratch<WARPS>& scratch, Walk<K>& mine_) {
+  constexpr int THREADS = 32 * WARPS;
+  const int per = (p.seqs + THREADS - 1) / THREADS, t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  const int lo = (int)min((long long)t * per, (long long)p.seqs), hi = min(lo + per, p.seqs);
+  long long mine = 0;
+  for (int b = lo; b < hi; ++b) mine += Costs(sequence(p, b), tl).head() * tl.heads;
+  long long upto = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long v = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += v;
+  }
+  if (lane == 31) scratch.sums[warp] = upto;
+  if (t == 0) scratch.b = -1;
+  __syncthreads();
+  long long total = 0;
+#pragma unroll
+  for (int i = 0; i < WARPS; ++i) {
+    if (i < warp) upto += scratch.sums[i];
+    total += scratch.sums[i];
+  }
+  const long long ctas = max(1ll, min((long long)gridDim.x, total / kShareCost));
+  const long long each = total / ctas, rest = total - each * ctas;
+  long long from = 0, to = 0;
+  if (blockIdx.x < ctas) {  // total * c / ctas without a product of 64 x 64 bits
+    from = each * blockIdx.x + rest * blockIdx.x / ctas;
+    to = each * (blockIdx.x + 1) + rest * (blockIdx.x + 1) / ctas;
+  }
+  if (from < to && upto - mine <= from && from < upto) {  // the thread whose sequences hold the start
+    long long at = upto - mine;
+    for (int b = lo; b < hi; ++b) {
+      const long long cost = Costs(sequence(p, b), tl).head() * tl.heads;
+      if (from < at + cost) {
+        scratch.b = b;
+        scratch.start = at;
+        break;
+      }
+      at += cost;
+    }
+  }
+  __syncthreads();
+  if (lane == 0) {
+    Walk<K> w{};
+    w.b = scratch.b;
+    if (w.b >= 0) {
+      w.to = to;
+      w.at = scratch.start;
+      w.share = (int)min(each, 0x7fffffffll);
+      const Sequence s = sequence(p, w.b);
+      w.take(s);
+      const Costs c(s, tl);
+      w.head = (int)((from - w.at) / c.head());
+      w.at += w.head * c.head();
+      int low = 0, high = c.items;  // the item that holds the start
+      while (high - low > 1) {
+        const int mid = (low + high) / 2;
+        if (c.before(mid) <= from - w.at) low = mid;
+        else high = mid;
+      }
+      w.item = low;
+      w.at += c.before(low);
+      w.enter(tl, from);
+      if (w.begin >= w.end) w.next(p, tl);
+    }
+    mine_ = w;
+  }
+  __syncwarp();
+}
+
+// What a CTA leaves for the join.  Slot 2c holds its first item where an earlier CTA has begun it, slot 2c + 1 its last one where a
+// later CTA ends it.
+struct Share {
+  int b, head, item;  // in slot 2c + 1; b = -1: none
+  short continues;    // slot 2c is filled; -1: the share has not one unit
+  short ends;         // slot 2c's item ends here
+};
+struct Parts {
+  float* acc;    // [slot][rows of an item][head_dim], not normalised
+  float2* ml;    // [slot][rows of an item]: maximum (log2 units) and sum
+  Share* share;  // per CTA
+};
+
+// Row r of an item: its token in the sequence and its query head; false where there is none
+__device__ __forceinline__ bool row_of(const PagedAttention& p, const Tiling& tl, int n, int head, int item, int tile, int r, int& token,
+                                       int& h) {
+  const int per = tl.tokens / tl.tiles, i = tl.by_group(r), kv = tl.subs == 1 ? head : head / tl.subs, sub = head - kv * tl.subs;
+  const int all = p.heads / p.kv_heads, in_group = sub * tl.group + (r - i * tl.group);
+  token = item * tl.tokens + tile * per + i;
+  h = kv * all + in_group;
+  return i < per && token < n && in_group < all;
 }
 
 // ---------------------------------------------------------------------------------- few rows per kv head: mma.sync
 
 constexpr int kKeys = 64;               // keys of a stage
+// What an item costs apart from its keys, in keys: the first load's way, the warps' join, the result.  200 sequences of up to 200
+// keys, 32 heads on 8 (us): 79 at 0, 34 at 128, 28 at 256, 30 at 512; where all are long it makes no difference.
+constexpr int kRowsFixed = 256;
 constexpr int kRowsThreads = 32 * 5;    // four warps of products and one that loads
-constexpr int kShareUnits = 2;          // stages that are worth a CTA
 
 template <int D_, int WM_>
 struct Rows {
@@ -55,20 +244,6 @@ struct Rows {
   static constexpr int EXCHANGE = WK > 1 ? 2 * 16 * D * 4 : 0;  // accumulators of two warps on their way to their neighbours
   static constexpr int SMEM = STAGES * STAGE + EXCHANGE + 1024;
   static_assert(SMEM <= 115712, "two CTAs per SM");
-};
-
-// What a CTA leaves for the join.  Slot 2c holds its first tile where an earlier CTA has begun it, slot 2c + 1 its last one where a
-// later CTA ends it.
-struct Share {
-  int b, kv_head;   // of the tile in slot 2c + 1; b = -1: none
-  int continues;    // slot 2c is filled
-  int ends;         // ... and its tile ends here
-};
-struct Parts {
-  float* acc;    // [slot][rows of a tile][head_dim], not normalised
-  float2* ml;    // [slot][rows of a tile]: maximum (log2 units) and sum
-  Share* share;  // per CTA
-  int rows;      // of a tile
 };
 
 __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2, int c3) {
@@ -101,100 +276,29 @@ __device__ __forceinline__ float quad_sum(float v) {
 }
 __device__ __forceinline__ void products_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }  // the four warps of products
 
-// Where a CTA's share stands: kv head `head` of sequence b, from stage `unit` on, `left` stages to go.
-struct Walk {
-  int b, head, unit, units;
-  long long left;
-  Sequence s;
-};
-template <int TR>
-__device__ __forceinline__ int units_of(const PagedAttention& p, const Sequence& s) {
-  return (long long)s.n * (p.heads / p.kv_heads) <= TR ? (s.keys + kKeys - 1) / kKeys : 0;
-}
-template <int TR>
-__device__ __forceinline__ void next_tile(Walk& w, const PagedAttention& p, int done) {
-  w.left -= done;
-  w.unit = 0;
-  if (++w.head < p.kv_heads) return;
-  w.head = 0;
-  w.units = 0;
-  while (w.left > 0 && w.units == 0 && ++w.b < p.seqs) {
-    w.s = sequence(p, w.b);
-    w.units = units_of<TR>(p, w.s);
-  }
-}
-
-// This CTA's share of all stages of all tiles, found by the whole block.  sums: a value per thread of the block and one more.
-template <int TR>
-__device__ Walk my_share(const PagedAttention& p, long long* sums, long long* found) {
-  const int per = (p.seqs + kRowsThreads - 1) / kRowsThreads, t = threadIdx.x, lane = t & 31, warp = t >> 5;
-  const int lo = min(t * per, p.seqs), hi = min(lo + per, p.seqs);
-  long long mine = 0;
-  for (int b = lo; b < hi; ++b) mine += (long long)units_of<TR>(p, sequence(p, b)) * p.kv_heads;
-  long long upto = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const long long v = __shfl_up_sync(0xffffffffu, upto, o);
-    if (lane >= o) upto += v;
-  }
-  if (lane == 31) sums[warp] = upto;
-  if (t == 0) found[0] = -1;
-  __syncthreads();
-  long long total = 0;
-#pragma unroll
-  for (int i = 0; i < kRowsThreads / 32; ++i) {
-    if (i < warp) upto += sums[i];
-    total += sums[i];
-  }
-  const long long ctas = min((long long)gridDim.x, (total + kShareUnits - 1) / kShareUnits);
-  long long from = 0, to = 0;
-  if (blockIdx.x < ctas) from = total * blockIdx.x / ctas, to = total * (blockIdx.x + 1) / ctas;
-  if (from < to && upto - mine <= from && from < upto) {  // the thread whose sequences hold the start
-    long long at = upto - mine;
-    for (int b = lo; b < hi; ++b) {
-      const long long u = (long long)units_of<TR>(p, sequence(p, b)) * p.kv_heads;
-      if (from < at + u) {
-        found[0] = b;
-        found[1] = from - at;
-        break;
-      }
-      at += u;
-    }
-  }
-  __syncthreads();
-  Walk w{(int)found[0], 0, 0, 0, to - from, {}};
-  if (w.b < 0) w.left = 0;
-  if (w.left > 0) {
-    w.s = sequence(p, w.b);
-    w.units = units_of<TR>(p, w.s);
-    w.head = (int)(found[1] / w.units);
-    w.unit = (int)(found[1] - (long long)w.head * w.units);
-  }
-  return w;
-}
-
 // Bound by the bandwidth of the cache: 64 keys are 32 KB (head dimension 128), which an SM gets in 1400 cycles, and take four
 // warps some 600.  So the legacy products, whose tiles are 16 rows high, do: the rows of single tokens fill no more.  A warp loads
 // 64 keys a stage by TMA, the boxes of several pages where they are smaller; where the rows fit one 16-row tile the four others
-// take 16 keys each and join their sums per tile, else they share the keys and have rows of their own.
+// take 16 keys each and join their sums per item, else they share the keys and have rows of their own.
 template <typename C>
 __global__ void __launch_bounds__(kRowsThreads, 2)
 paged_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const PagedAttention p,
-                  const Parts parts, const FastDiv by_group) {
+                  const Parts parts, const __grid_constant__ Tiling tl) {
   constexpr int D = C::D, WK = C::WK, TR = C::TR;
   extern __shared__ __align__(1024) uint8_t smem[];
   float* exchange = reinterpret_cast<float*>(smem + C::STAGES * C::STAGE);
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::STAGES * C::STAGE + C::EXCHANGE);
   uint64_t* empty = full + C::STAGES;
-  long long* sums = reinterpret_cast<long long*>(empty + C::STAGES);
-  long long* found = sums + kRowsThreads / 32;
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(found + 2);
-  float2* stats = reinterpret_cast<float2*>(found + 3);  // [warp][16 rows]
+  auto* scratch = reinterpret_cast<ShareScratch<kRowsThreads / 32>*>(empty + C::STAGES);
+  auto* walks = reinterpret_cast<Walk<kKeys>*>(scratch + 1);
+  float2* stats = reinterpret_cast<float2*>(walks + kRowsThreads / 32);  // [warp][16 rows]
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(stats + 4 * 16);
+  static_assert(C::STAGES * 16 + sizeof(*scratch) + sizeof(*walks) * kRowsThreads / 32 + 4 * 16 * sizeof(float2) + 4 <= 1024);
   const int warp = (int)warp_uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (smem_u32(smem) & 1023) {  // the 128-byte swizzle repeats every 1024 bytes
     if (threadIdx.x == 0) {
       bad_argument(p.status);
-      parts.share[blockIdx.x] = Share{-1, 0, 0, 0};
+      parts.share[blockIdx.x] = Share{-1, 0, 0, -1, 0};
     }
     return;
   }
@@ -210,19 +314,18 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
   }
   pdl_trigger();
   pdl_wait();
-  Walk w = my_share<TR>(p, sums, found);
-  const int group = p.heads / p.kv_heads;
+  Walk<kKeys>& w = walks[warp];
+  my_share(p, tl, *scratch, w);
   Ring<C::STAGES> ring;
 
   if (warp == 4) {
     // ------------------------------------------------------------------ loads
     const int shift = p.page_shift, box = min(kKeys, 1 << shift), boxes = kKeys / box;
-    while (w.left > 0) {
-      const int end = (int)min((long long)w.units, w.unit + w.left);
+    for (; w.valid(); w.next(p, tl, lane)) {
       const int* table = p.page_table + (long long)w.b * p.table_pitch;
-      const int used = (int)(((long long)w.s.keys + (1 << shift) - 1) >> shift);
+      const int used = (int)(((long long)w.keys + (1 << shift) - 1) >> shift);
       int held = 0, have = 0, page = 0;  // lane i: page held + i, for i < have
-      for (int u = w.unit; u < end; ++u) {
+      for (int u = w.begin; u < w.end; ++u) {
         const int key = u * kKeys, first = key >> shift, count = min(boxes, used - first);
         if (first < held || first + count > held + have) {
           held = first;
@@ -256,7 +359,6 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
         ring.next();
       }
       if (__any_sync(0xffffffffu, *abort_flag != 0)) break;
-      next_tile<TR>(w, p, end - w.unit);
     }
   } else {
     // ------------------------------------------------------------------ products
@@ -266,21 +368,22 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
     const int key0 = wk * (kKeys / WK), quad = lane >> 2, pair = (lane & 3) * 2;
     const float scale = p.scale * 1.4426950408889634f;
     bool dead = false;
-    Share share{-1, 0, 0, 0};
-    bool first_tile = true;
-    while (w.left > 0) {
-      const int begin = w.unit, end = (int)min((long long)w.units, w.unit + w.left), rows = w.s.n * group;
-      const int cached = w.s.keys - w.s.n;
+    Share share{-1, 0, 0, -1, 0};
+    bool first_item = true;
+    for (; w.valid(); w.next(p, tl, lane)) {
+      const int least = w.cached + w.item * tl.tokens + 1;  // keys that the first token sees
       // queries of rows quad and quad + 8, and how many keys these see
       uint32_t q[D / 16][4];
       int sees[2];
       long long to[2];  // their rows of the result
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const int r = wm * 16 + quad + 8 * i, token = by_group(min(r, rows - 1)), h = w.head * group + (min(r, rows - 1) - token * group);
-        const bf16* src = p.q + (w.s.first + token) * p.q_token + h * p.q_head + pair;
-        sees[i] = cached + token + 1;
-        to[i] = r < rows ? ((long long)(w.s.first + token) * p.heads + h) * D : -1;
+        int token, h;
+        const bool there = row_of(p, tl, w.n, w.head, w.item, 0, wm * 16 + quad + 8 * i, token, h);
+        sees[i] = there ? w.cached + token + 1 : least;
+        to[i] = there ? ((long long)(w.first + token) * p.heads + h) * D : -1;
+        if (!there) token = w.item * tl.tokens, h = w.head / tl.subs * (p.heads / p.kv_heads);  // a row that exists
+        const bf16* src = p.q + (w.first + token) * p.q_token + h * p.q_head + pair;
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
           q[kk][i] = *reinterpret_cast<const uint32_t*>(src + kk * 16);
@@ -290,7 +393,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
       float o[D / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 #pragma unroll
       for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-      for (int u = begin; u < end; ++u) {
+      for (int u = w.begin; u < w.end; ++u) {
         if (!dead && !mbar_wait(&full[ring.s], ring.ph, abort_flag)) {
           *abort_flag = 1;
           atomicCAS(p.status, 0, kStatusMmaTimeout);
@@ -311,7 +414,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
             mma16816(s[2 * g], q[kk], k[0], k[1]);
             mma16816(s[2 * g + 1], q[kk], k[2], k[3]);
           }
-        if (at + KG * 16 > cached + 1) {  // beyond what the first token sees
+        if (at + KG * 16 > least) {  // beyond what the first token sees
 #pragma unroll
           for (int i = 0; i < 2 * KG; ++i)
 #pragma unroll
@@ -346,11 +449,11 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
 #pragma unroll
           for (int i = 0; i < D / 8; ++i) o[i][0] *= f[0], o[i][1] *= f[0], o[i][2] *= f[1], o[i][3] *= f[1];
         }
-        const bool ragged = at + KG * 16 > w.s.keys;  // what lies behind the last key may be no numbers: taken as zeros
+        const bool ragged = at + KG * 16 > w.keys;  // what lies behind the last key may be no numbers: taken as zeros
 #pragma unroll
         for (int g = 0; g < KG; ++g) {
           const uint32_t a[4] = {pr[2 * g][0], pr[2 * g][1], pr[2 * g + 1][0], pr[2 * g + 1][1]};
-          const int left = w.s.keys - (at + g * 16) - pair;  // of the keys from this lane's first on
+          const int left = w.keys - (at + g * 16) - pair;  // of the keys from this lane's first on
           const uint32_t keep0 = (left > 0 ? 0xffffu : 0u) | (left > 1 ? 0xffff0000u : 0u);
           const uint32_t keep1 = (left > 8 ? 0xffffu : 0u) | (left > 9 ? 0xffff0000u : 0u);
 #pragma unroll
@@ -413,7 +516,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
           products_sync();
         }
       }
-      const bool starts = begin == 0, ends = end == w.units;
+      const bool starts = w.begin == 0, ends = w.end == w.units;
       if (wk == 0) {
         if (starts && ends) {
 #pragma unroll
@@ -437,10 +540,9 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
           }
         }
       }
-      if (starts && !ends) share.b = w.b, share.kv_head = w.head;
-      if (!starts && first_tile) share.continues = 1, share.ends = ends;
-      first_tile = false;
-      next_tile<TR>(w, p, end - begin);
+      if (starts && !ends) share.b = w.b, share.head = w.head, share.item = w.item;
+      if (first_item) share.continues = !starts, share.ends = ends;
+      first_item = false;
     }
     if (threadIdx.x == 0) parts.share[blockIdx.x] = share;
   }
@@ -452,52 +554,58 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
   }
 }
 
-// Joins the parts of tiles that several CTAs had, writes zeros to rows that are nobody's and reports what is wrong with the
-// sequences.  Block (c, y) has the tile that CTA c began, rows y, y + 8 * gridDim.y ..., one per warp.
-template <int D>
-__global__ void __launch_bounds__(256) paged_join_kernel(const PagedAttention p, const Parts parts, int ctas) {
+// Joins the parts of items that several CTAs had, writes zeros to rows that are nobody's and reports what is wrong with the
+// sequences.  Block (c, y) has the item that CTA c began, and of its rows as many at a time as it has groups of WPR warps; the
+// warps of a group share the parts.  Few rows come in many parts (a cache of 4000 keys over the whole GPU in 30), so eight warps
+// take a row together there; many rows come in two or three, and a warp takes each.
+template <int D, int WPR>
+__global__ void __launch_bounds__(256) paged_join_kernel(const PagedAttention p, const Parts parts, const __grid_constant__ Tiling tl) {
+  constexpr int E = D / 32, ROWS = 8 / WPR;  // columns of a lane, rows of a block at a time
+  __shared__ float sums[WPR > 1 ? WPR : 1][D + 2];
   pdl_trigger();
   pdl_wait();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = blockIdx.x;
-  const int group = p.heads / p.kv_heads;
-  if (blockIdx.y == 0) {  // sequences c, c + gridDim.x ... and a share of the rows behind the last
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = blockIdx.x, ctas = gridDim.x, rows = tl.height * tl.tiles;
+  const Share mine = parts.share[c];
+  if (blockIdx.y == 0) {  // sequences c, c + ctas ... and a share of the rows behind the last
     auto clear = [&](long long lo, long long hi) {
       lo = max(lo, 0ll);
       hi = min(hi, (long long)p.tokens);
       const long long per_row = (long long)p.heads * D / 8;
       for (long long i = lo * per_row + threadIdx.x; i < hi * per_row; i += 256) reinterpret_cast<uint4*>(p.out)[i] = make_uint4(0, 0, 0, 0);
     };
-    for (int b = c; b < p.seqs; b += gridDim.x) {
+    for (int b = c; b < p.seqs; b += ctas) {
       if (sequence(p, b).bad) {
         if (threadIdx.x == 0) bad_argument(p.status);
         clear(p.offsets[b], p.offsets[b + 1]);
       }
     }
     if (c == 0 && threadIdx.x == 0 && p.offsets[0] != 0) bad_argument(p.status);
-    for (long long r = (long long)p.offsets[p.seqs] + c; r < p.tokens; r += gridDim.x) clear(r, r + 1);
+    for (long long r = max(0ll, (long long)p.offsets[p.seqs]) + c; r < p.tokens; r += ctas) clear(r, r + 1);
   }
-  if (c >= ctas) return;
-  const Share mine = parts.share[c];
   if (mine.b < 0) return;
   const Sequence s = sequence(p, mine.b);
-  int last = c;  // the CTA that ends the tile
+  int last = c;  // the CTA that ends the item
   for (bool more = true; more;) {
     const int i = last + 1 + lane;
-    const bool stop = i >= ctas || !parts.share[i].continues || parts.share[i].ends;
+    const bool stop = i >= ctas || parts.share[i].continues == 0 || (parts.share[i].continues > 0 && parts.share[i].ends);
     const unsigned at = __ballot_sync(0xffffffffu, stop);
     more = at == 0;
     last += more ? 32 : __ffs(at);
   }
   last = min(last, ctas - 1);
-  constexpr int E = D / 32;
-  for (int r = blockIdx.y * 8 + warp; r < s.n * group; r += 8 * gridDim.y) {
+  const int sub = warp % WPR;
+  for (int r = blockIdx.y * ROWS + warp / WPR; r < rows; r += ROWS * gridDim.y) {
+    int token, h;
+    if (!row_of(p, tl, s.n, mine.head, mine.item, r / tl.height, r % tl.height, token, h)) continue;  // all warps of the row
     float top = -INFINITY, sum = 0.f, acc[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] = 0.f;
-    for (int base = c; base <= last; base += 32) {
-      const int i = base + lane;
+    // this warp's parts are those of CTAs c + sub, c + sub + WPR ..., 32 at a time
+    for (int base = c + sub; base <= last; base += 32 * WPR) {
+      const int i = base + lane * WPR;
       const long long slot = i == c ? 2ll * c + 1 : 2ll * i;
-      const float2 t = i <= last ? parts.ml[slot * parts.rows + r] : make_float2(-INFINITY, 0.f);
+      const bool has = i == c || (i <= last && parts.share[i].continues > 0);
+      const float2 t = has ? parts.ml[slot * rows + r] : make_float2(-INFINITY, 0.f);
       float most = t.x;
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
@@ -509,68 +617,450 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedAttention p,
       top = top2;
 #pragma unroll
       for (int e = 0; e < E; ++e) acc[e] *= f;
-      const int n = min(32, last + 1 - base);
+      const int n = min(32, (last - base) / WPR + 1);
 #pragma unroll 4
       for (int k = 0; k < n; ++k) {
         const float wk = __shfl_sync(0xffffffffu, mw, k);
-        const long long from = (base + k == c ? 2ll * c + 1 : 2ll * (base + k)) * parts.rows + r;
+        const int j = base + k * WPR;
+        const long long from = (j == c ? 2ll * c + 1 : 2ll * j) * rows + r;
+        if (wk > 0.f) {  // a part that saw none of the row's keys, or a share without units, has nothing written
 #pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] += wk * parts.acc[from * D + e * 32 + lane];
+          for (int e = 0; e < E; ++e) acc[e] += wk * parts.acc[from * D + e * 32 + lane];
+        }
       }
     }
-    const int token = r / group, h = mine.kv_head * group + (r - token * group);
-    const float inv = sum > 0.f ? 1.f / sum : 0.f;
+    if constexpr (WPR > 1) {
+      if (lane == 0) sums[sub][D] = top, sums[sub][D + 1] = sum;
 #pragma unroll
-    for (int e = 0; e < E; ++e)
-      p.out[((long long)(s.first + token) * p.heads + h) * D + e * 32 + lane] = __float2bfloat16(acc[e] * inv);
+      for (int e = 0; e < E; ++e) sums[sub][e * 32 + lane] = acc[e];
+      __syncthreads();
+      if (sub == 0) {
+#pragma unroll
+        for (int i = 1; i < WPR; ++i) top = fmaxf(top, sums[i][D]);
+        sum = 0.f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] = 0.f;
+#pragma unroll
+        for (int i = 0; i < WPR; ++i) {
+          const float f = fast_exp2(sums[i][D] - (top == -INFINITY ? 0.f : top));
+          sum += sums[i][D + 1] * f;
+#pragma unroll
+          for (int e = 0; e < E; ++e) acc[e] += sums[i][e * 32 + lane] * f;
+        }
+      }
+    }
+    if (sub == 0) {
+      const float inv = sum > 0.f ? 1.f / sum : 0.f;
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        p.out[((long long)(s.first + token) * p.heads + h) * D + e * 32 + lane] = __float2bfloat16(acc[e] * inv);
+    }
+    if constexpr (WPR > 1) __syncthreads();
   }
 }
 
-// ---------------------------------------------------------------------------------- many rows
+// ---------------------------------------------------------------------------------- many rows: tcgen05
 
-// The sequences whose rows are too many for the kernel above.  One warp per query row: its lanes share the head dimension, keys one after the other with the running maximum and sum.
+// As kRowsFixed.  48 prompts of up to 1024 tokens, 12 heads of 64 (us): 147 at 0, 116 at 128, 112 at 256, 108.5 at 384, 110 at 512
+constexpr int kChunkFixed = 384;
+constexpr int kChunkThreads = 32 * 12;  // loads; products of either query tile; a spare; four softmax warps per query tile
+
 template <int D>
-__global__ void __launch_bounds__(128) paged_attention_kernel(const PagedAttention p, int above) {
-  constexpr int E = D / 32;
+struct Chunk {
+  static constexpr int PANELS = D / 64;           // 128-byte panels along the head dimension
+  static constexpr int TILE_BYTES = kBM * D * 2;  // 128 rows of Q, K or V
+  static constexpr int K_STAGES = D == 128 ? 3 : 4, V_STAGES = D == 128 ? 2 : 4;
+  static constexpr int SMEM = (2 + K_STAGES + V_STAGES) * TILE_BYTES + 1536;
+  // tensor memory: S and O of both query tiles; D = 64 has room for P beside S, D = 128 writes P over S
+  static constexpr bool P_APART = D == 64;
+  static constexpr int S_COL = 0, O_COL = 2 * kBM, P_COL = P_APART ? 2 * kBM + 2 * D : S_COL;
+  static constexpr int P_TILE = P_APART ? 64 : kBM;  // columns from one query tile's P to the other's
+  static constexpr int TMEM_COLS = 512;
+  static_assert(P_COL + 2 * 64 <= TMEM_COLS && O_COL + 2 * D <= TMEM_COLS && SMEM <= 232448, "one CTA per SM");
+};
+
+// Units of an item that its query tile x has to do: those of this share up to the last one that a row of the tile sees
+__device__ __forceinline__ int tile_end(const Walk<kBM>& w, const Tiling& tl, int x) {
+  const int per = tl.tokens / 2, first = w.item * tl.tokens + x * per;
+  if (first >= w.n) return w.begin;
+  const int sees = w.cached + min(first + per, w.n);
+  return max(w.begin, min(w.end, (sees + kBM - 1) / kBM));
+}
+
+// One CTA per SM goes through items of two query tiles of 128 rows, which share the K and V tiles; each has four softmax warps with
+// a query row per thread and a warp that issues its products, so that one tile's exponentials run under the other's products.  K
+// and V come page by page; keys behind the last one are masked and their values, which may be no numbers, replaced by zeros in
+// shared memory by the softmax warps before they hand on the weights.
+template <int D>
+__global__ void __launch_bounds__(kChunkThreads, 1)
+paged_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
+                   const __grid_constant__ CUtensorMap tmap_v, const PagedAttention p, const Parts parts, const __grid_constant__ Tiling tl) {
+  using C = Chunk<D>;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint8_t* sQ = smem;  // two tiles
+  uint8_t* sK = sQ + 2 * C::TILE_BYTES;
+  uint8_t* sV = sK + C::K_STAGES * C::TILE_BYTES;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sV + C::V_STAGES * C::TILE_BYTES);
+  uint64_t* q_full = bars;        // one per query tile, as the next five
+  uint64_t* q_empty = bars + 2;
+  uint64_t* s_full = bars + 4;
+  uint64_t* s_free = bars + 6;    // four warps: S is in registers (P_APART)
+  uint64_t* p_full = bars + 8;    // four warps
+  uint64_t* pv_done = bars + 10;  // O += P V retired: O stable, P free
+  uint64_t* k_full = bars + 12;   // K_STAGES each
+  uint64_t* k_empty = k_full + C::K_STAGES;
+  uint64_t* v_full = k_empty + C::K_STAGES;  // V_STAGES each
+  uint64_t* v_empty = v_full + C::V_STAGES;
+  uint64_t* bars_end = v_empty + C::V_STAGES;
+  auto* scratch = reinterpret_cast<ShareScratch<kChunkThreads / 32>*>(bars_end);
+  auto* walks = reinterpret_cast<Walk<kBM>*>(scratch + 1);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(walks + kChunkThreads / 32);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  static_assert((12 + 2 * (C::K_STAGES + C::V_STAGES)) * 8 + sizeof(*scratch) + sizeof(*walks) * kChunkThreads / 32 + 8 <= 1536);
+
+  const int warp = (int)warp_uniform(threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (smem_u32(smem) & 1023) {  // the 128-byte swizzle repeats every 1024 bytes
+    if (threadIdx.x == 0) {
+      bad_argument(p.status);
+      parts.share[blockIdx.x] = Share{-1, 0, 0, -1, 0};
+    }
+    return;
+  }
+  if (threadIdx.x == 0) {
+    tma_prefetch_desc(&tmap_q);
+    tma_prefetch_desc(&tmap_k);
+    tma_prefetch_desc(&tmap_v);
+    for (uint64_t* b = bars; b < bars_end; ++b)
+      mbar_init(b, (b >= s_free && b < pv_done) ? 4 : ((b >= k_empty && b < v_full) || b >= v_empty) ? 2 : 1);
+    *abort_flag = 0;
+    mbar_fence_init();
+  }
   pdl_trigger();
   pdl_wait();
-  const int lane = threadIdx.x & 31;
-  const long long w = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (w >= (long long)p.tokens * p.heads) return;
-  const int row = (int)(w / p.heads), h = (int)(w - (long long)row * p.heads), hk = h / (p.heads / p.kv_heads);
-  const int b = sequence_of(p.offsets, p.seqs, row, lane);
-  const Sequence seq = sequence(p, b);
-  if (row < seq.first || row >= seq.first + seq.n || (long long)seq.n * (p.heads / p.kv_heads) <= above) return;
-  const long long keys = seq.keys - seq.n + (row - seq.first) + 1;
-  float q[E], o[E], m = -INFINITY, l = 0.f;
-#pragma unroll
-  for (int i = 0; i < E; ++i) {
-    q[i] = __bfloat162float(p.q[row * p.q_token + h * p.q_head + lane * E + i]) * p.scale * 1.4426950408889634f;
-    o[i] = 0.f;
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, C::TMEM_COLS);
+    tmem_relinquish();
   }
-  for (long long j = 0; j < keys; ++j) {
-    const int page = p.page_table[(long long)b * p.table_pitch + (j >> p.page_shift)];
-    if (page < 0 || page >= p.pages) {
-      bad_argument(p.status);
-      continue;
+  Walk<kBM>& w = walks[warp];
+  tc_fence_before();
+  my_share(p, tl, *scratch, w);  // synchronises the block
+  tc_fence_after();
+  const uint32_t tmem_base = warp_uniform(*tmem_slot);
+  const int per = tl.tokens / 2;  // tokens of a query tile
+
+  if (warp < 4) {
+    give_registers<96, 200>();
+    if (warp == 0) {
+      // ---------------------------------------------------------------- loads
+      const int shift = p.page_shift, box = min(kBM, 1 << shift), boxes = kBM / box;
+      Ring<C::K_STAGES> ks;
+      Ring<C::V_STAGES> vs;
+      int nq[2] = {0, 0};  // loads of each query tile's buffer
+      bool ok = true;
+      auto free_slot = [&](uint64_t* bar, uint32_t parity) {  // the same answer in all lanes
+        const bool got = mbar_wait(bar, parity, abort_flag);
+        ok = __all_sync(0xffffffffu, got);
+        return ok;
+      };
+      for (; ok && w.valid(); w.next(p, tl, lane)) {
+        const int* table = p.page_table + (long long)w.b * p.table_pitch;
+        const int used = (int)(((long long)w.keys + (1 << shift) - 1) >> shift);
+        const int kv = w.head / tl.subs, h0 = kv * (p.heads / p.kv_heads) + (w.head - kv * tl.subs) * tl.group;
+        int held = 0, have = 0, page = 0;  // lane i: page held + i, for i < have
+        for (int x = 0; x < 2 && ok; ++x) {
+          if (tile_end(w, tl, x) == w.begin) continue;
+          if (!free_slot(&q_empty[x], (nq[x] & 1) ^ 1u)) break;
+          if (lane == 0) {
+            mbar_arrive_expect_tx(&q_full[x], per * tl.group * D * 2);
+#pragma unroll
+            for (int c = 0; c < C::PANELS; ++c)
+              tma_load_3d(sQ + x * C::TILE_BYTES + c * (kBM * 128), &tmap_q, &q_full[x], c * 64, h0, w.first + w.item * tl.tokens + x * per);
+          }
+          ++nq[x];
+        }
+        for (int u = w.begin; ok && u < w.end; ++u) {
+          const int key = u * kBM, first = key >> shift, count = min(boxes, used - first), at = key & ((1 << shift) - 1);
+          if (first < held || first + count > held + have) {
+            held = first;
+            have = min(32, used - first);
+            if (lane < have) {
+              page = table[first + lane];
+              if (page < 0 || page >= p.pages) {
+                bad_argument(p.status);
+                page = 0;
+              }
+            }
+          }
+          const int mine = __shfl_sync(0xffffffffu, page, (first - held + lane) & 31);
+          auto load = [&](uint8_t* dst, const CUtensorMap* map, uint64_t* bar) {
+            if (lane == 0) mbar_arrive_expect_tx(bar, count * box * D * 2);
+            __syncwarp();
+            if (lane < count) {
+#pragma unroll
+              for (int c = 0; c < C::PANELS; ++c) tma_load_4d(dst + c * (kBM * 128) + lane * box * 128, map, bar, c * 64, kv, at, mine);
+            }
+          };
+          if (!free_slot(&k_empty[ks.s], ks.ph ^ 1u)) break;
+          load(sK + ks.s * C::TILE_BYTES, &tmap_k, &k_full[ks.s]);
+          if (!free_slot(&v_empty[vs.s], vs.ph ^ 1u)) break;
+          load(sV + vs.s * C::TILE_BYTES, &tmap_v, &v_full[vs.s]);
+          ks.next();
+          vs.next();
+        }
+      }
+      if (!ok && lane == 0) {
+        *abort_flag = 1;
+        atomicCAS(p.status, 0, kStatusProducerTimeout);
+      }
+    } else if (warp < 3) {
+      // ---------------------------------------------------------------- S = Q K^T and O += P V of one query tile
+      if (elect_one()) {
+        const int x = warp - 1;
+        constexpr uint32_t idesc = make_instr_desc(1, kMajorK, kMajorMN, kBM, D);
+        const DescHalves dq_ = desc_halves(smem_u32(sQ) + x * C::TILE_BYTES, 16, 1024), dk_ = desc_halves(smem_u32(sK), 16, 1024);
+        const DescHalves dv_ = desc_halves(smem_u32(sV), kBM * 128, 1024);
+        const uint32_t s_col = tmem_base + C::S_COL + x * kBM, p_col = tmem_base + C::P_COL + x * C::P_TILE;
+        const uint32_t o_col = tmem_base + C::O_COL + x * D;
+        bool ok = true;
+        Ring<C::K_STAGES> ks;
+        Ring<C::V_STAGES> vs;
+        uint32_t ph = 0;  // of the unit whose P is awaited
+        uint32_t nq = 0;  // query tiles so far
+        auto issue_s = [&](int u, int end) {  // S of unit u of the item at hand
+          ok = ok && mbar_wait(&k_full[ks.s], ks.ph, abort_flag) && (u > w.begin || mbar_wait(&q_full[x], nq & 1, abort_flag));
+          if (!ok) return;
+          tc_fence_after();
+          scores<D, false>(s_col, dq_, 0, dk_, ks.s * C::TILE_BYTES);
+          umma_commit(&s_full[x]);
+          umma_commit(&k_empty[ks.s]);
+          if (u == end - 1) {
+            umma_commit(&q_empty[x]);
+            ++nq;
+          }
+          ks.next();
+        };
+        auto skip = [&]() {  // a pair of K and V tiles that this query tile does not see: passed on once it has arrived
+          ok = ok && mbar_wait(&k_full[ks.s], ks.ph, abort_flag);
+          if (ok) mbar_arrive(&k_empty[ks.s]);
+          ok = ok && mbar_wait(&v_full[vs.s], vs.ph, abort_flag);
+          if (ok) mbar_arrive(&v_empty[vs.s]);
+          ks.next();
+          vs.next();
+        };
+        for (; ok && w.valid(); w.next(p, tl)) {
+          const int end = tile_end(w, tl, x);
+          if (end > w.begin) issue_s(w.begin, end);  // the S before has been read: P of it has been multiplied
+          for (int u = w.begin; u < end && ok; ++u) {
+            if (C::P_APART && u + 1 < end) {
+              ok = mbar_wait(&s_free[x], ph, abort_flag);
+              issue_s(u + 1, end);
+            }
+            ok = ok && mbar_wait(&v_full[vs.s], vs.ph, abort_flag) && mbar_wait(&p_full[x], ph, abort_flag);
+            if (!ok) break;
+            tc_fence_after();
+#pragma unroll
+            for (int kk = 0; kk < kBM / 16; ++kk)
+              umma_ts_h(o_col, p_col + kk * 8, dv_, vs.s * C::TILE_BYTES + kk * (16 * 128), idesc, (u > w.begin || kk > 0) ? 1u : 0u);
+            umma_commit(&pv_done[x]);
+            umma_commit(&v_empty[vs.s]);
+            vs.next();
+            if (!C::P_APART && u + 1 < end) issue_s(u + 1, end);  // over the P just read: the tensor core keeps the order
+            ph ^= 1u;
+          }
+          for (int u = end; u < w.end && ok; ++u) skip();
+        }
+        if (!ok) {
+          *abort_flag = 1;
+          atomicCAS(p.status, 0, kStatusMmaTimeout);
+        }
+      }
     }
-    const int at = (int)(j & ((1 << p.page_shift) - 1));
-    const bf16* k = p.k_pages + page * p.k_page + at * p.k_row + hk * p.k_head + lane * E;
-    const bf16* v = p.v_pages + page * p.v_page + at * p.v_row + hk * p.v_head + lane * E;
-    float s = 0.f;
+  } else {
+    // ------------------------------------------------------------------ softmax, stores
+    // Quadrant = warp & 3 (query rows), x = which query tile.  A wait that gives up raises the abort flag for all roles
+    // and the warp goes on (its lanes stay together); nothing is stored then.
+    take_registers<96, 200>();
+    const int quad = warp & 3;
+    const int x = (warp - 4) >> 2;
+    const int row_in_tile = quad * 32 + lane;
+    const uint32_t lane_base = tmem_base + ((uint32_t)(quad * 32) << 16);
+    const uint32_t s_col = lane_base + C::S_COL + x * kBM, p_col = lane_base + C::P_COL + x * C::P_TILE;
+    const uint32_t o_col = C::O_COL + x * D;
+    const float scale_log2 = p.scale * 1.4426950408889634f;
+    const f32x2 s2 = pack2(scale_log2, scale_log2);
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+      if (!mbar_wait(bar, parity, abort_flag)) *abort_flag = 1;
+      __syncwarp();  // the tensor-memory accesses that follow take the whole warp at once
+    };
+    uint32_t ph = 0;      // of the unit at hand: s_full, s_free, p_full, pv_done
+    uint32_t passed = 0;  // units of the items before
+    Share share{-1, 0, 0, -1, 0};
+    bool first_item = true;
+    for (; w.valid(); w.next(p, tl, lane)) {
+      const int end = tile_end(w, tl, x), keys = w.keys;
+      const int first = w.item * tl.tokens + x * per;
+      const int least = w.cached + first + 1;                                // keys that the first row sees
+      const int sees = w.cached + min(first + tl.by_group(row_in_tile), w.n - 1) + 1;  // and this one
+      float m_used = -INFINITY;  // reference max of the exponentials accumulated so far (log2 domain)
+      float l = 0.f;
+      for (int u = w.begin; u < end; ++u) {
+        wait(&s_full[x], ph);
+        tc_fence_after();
+        float sc[kBM];
 #pragma unroll
-    for (int i = 0; i < E; ++i) s += q[i] * __bfloat162float(k[i]);
+        for (int c = 0; c < 4; ++c) tmem_ld_32x32(s_col + c * 32, *reinterpret_cast<float(*)[32]>(&sc[c * 32]));
+        tmem_ld_wait();
+        if (C::P_APART) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&s_free[x]);
+        }
+        if ((u + 1) * kBM > least) {
+          const int mine = sees - u * kBM;
 #pragma unroll
-    for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-    const float m2 = fmaxf(m, s), a = m2 == -INFINITY ? 1.f : exp2f(m - m2), e = m2 == -INFINITY ? 0.f : exp2f(s - m2);
-    l = l * a + e;
+          for (int i = 0; i < kBM; ++i)
+            if (i >= mine) sc[i] = -INFINITY;
+        }
+        if ((u + 1) * kBM > keys) {  // what lies behind the last key may be no numbers
+          const uint32_t nth = passed + (uint32_t)(u - w.begin), stage = nth % C::V_STAGES;
+          wait(&v_full[stage], (nth / C::V_STAGES) & 1);
+          if (row_in_tile >= keys - u * kBM) {
 #pragma unroll
-    for (int i = 0; i < E; ++i) o[i] = o[i] * a + e * __bfloat162float(v[i]);
-    m = m2;
+            for (int c = 0; c < C::PANELS * 8; ++c)
+              *reinterpret_cast<uint4*>(sV + stage * C::TILE_BYTES + (c >> 3) * (kBM * 128) + row_in_tile * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_shared();
+        }
+        // row maximum of the raw scores (the scale is positive), four independent chains
+        float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int i = 0; i < kBM; i += 8) {
+#pragma unroll
+          for (int t = 0; t < 4; ++t) mx4[t] = fmaxf(mx4[t], fmaxf(sc[i + 2 * t], sc[i + 2 * t + 1]));
+        }
+        const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * scale_log2;
+        const float m_new = fmaxf(m_used, mx);
+        const bool need = u == w.begin || m_new - m_used > kRescaleThreshold;
+        if (__any_sync(0xffffffffu, need)) {
+          if (u > w.begin) {
+            // O may only be touched between two products: the one before must have retired, the next one cannot start
+            // before this warp delivered its P
+            wait(&pv_done[x], ph ^ 1u);
+            tc_fence_after();
+            const float alpha = m_new == -INFINITY ? 1.f : fast_exp2(m_used - m_new);
+            l *= alpha;
+#pragma unroll 1
+            for (int c = 0; c < D / 32; ++c) {
+              float o[32];
+              tmem_ld_32x32(lane_base + o_col + c * 32, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] *= alpha;
+              tmem_st_32x32(lane_base + o_col + c * 32, o);
+            }
+            tmem_st_wait();
+          }
+          m_used = m_new;
+        }
+        const float neg_m = m_used == -INFINITY ? 0.f : -m_used;
+        const f32x2 nm2 = pack2(neg_m, neg_m);
+        f32x2 sums[2] = {pack2(0.f, 0.f), pack2(0.f, 0.f)};
+        // exponentials, packed to bf16 pairs; their sum is that of the unrounded ones
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) {
+            float e0, e1;
+            unpack2(fma2(pack2(sc[c * 32 + i], sc[c * 32 + i + 1]), s2, nm2), e0, e1);
+            e0 = fast_exp2(e0);
+            e1 = fast_exp2(e1);
+            pk[i >> 1] = pack_bf16x2(e0, e1);
+            sums[(i >> 1) & 1] = add2(sums[(i >> 1) & 1], pack2(e0, e1));
+          }
+          if (C::P_APART && c == 0) wait(&pv_done[x], ph ^ 1u);  // the P before this one
+          tmem_st_32x16(p_col + c * 16, pk);
+        }
+        float sum0, sum1;
+        unpack2(add2(sums[0], sums[1]), sum0, sum1);
+        l += sum0 + sum1;
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[x]);
+        ph ^= 1u;
+      }
+      passed += (uint32_t)(w.end - w.begin);
+      const bool starts = w.begin == 0, ends = w.end == w.units;
+      const long long slot = 2 * (long long)blockIdx.x + (starts ? 1 : 0);
+      const long long part = slot * (2 * kBM) + x * kBM;
+      if (end > w.begin) {
+        // normalise and write out, or leave the part for the join.  The next item's first product overwrites O only after
+        // these warps delivered its P.
+        wait(&pv_done[x], ph ^ 1u);
+        tc_fence_after();
+        if (__any_sync(0xffffffffu, *abort_flag != 0)) break;
+        const float inv = l > 0.f ? 1.f / l : 0.f;
+#pragma unroll
+        for (int c0 = 0; c0 < D; c0 += 64) {  // all loads of 64 columns first: they take as long as one
+          float v[2][2][16];
+#pragma unroll
+          for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+              tmem_ld_16x256b_x4(tmem_base + o_col + ((uint32_t)(quad * 32 + hh * 16) << 16) + c0 + c * 32, v[hh][c]);
+          tmem_ld_wait();
+#pragma unroll
+          for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {  // rows lane >> 2 and that + 8
+              const int r = hh * 16 + half * 8 + (lane >> 2);
+              const float f = __shfl_sync(0xffffffffu, inv, r);
+              int token, h;
+              const bool there = row_of(p, tl, w.n, w.head, w.item, x, quad * 32 + r, token, h);
+              if (starts && ends) {
+                bf16* dst = p.out + ((long long)(w.first + token) * p.heads + h) * D + c0 + (lane & 3) * 8;
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                  uint32_t t[4];
+#pragma unroll
+                  for (int k = 0; k < 4; ++k) t[k] = pack_bf16x2(v[hh][c][4 * k + 2 * half] * f, v[hh][c][4 * k + 2 * half + 1] * f);
+                  quad_transpose(t, lane);
+                  if (there) *reinterpret_cast<uint4*>(dst + c * 32) = make_uint4(t[0], t[1], t[2], t[3]);
+                }
+              } else if (there) {
+                float* dst = parts.acc + (part + quad * 32 + r) * D + c0 + (lane & 3) * 2;
+#pragma unroll
+                for (int c = 0; c < 2; ++c)
+#pragma unroll
+                  for (int k = 0; k < 4; ++k)
+                    *reinterpret_cast<float2*>(dst + c * 32 + k * 8) = make_float2(v[hh][c][4 * k + 2 * half], v[hh][c][4 * k + 2 * half + 1]);
+              }
+            }
+        }
+      }
+      if (!(starts && ends)) parts.ml[part + row_in_tile] = make_float2(m_used, l);
+      if (starts && !ends) share.b = w.b, share.head = w.head, share.item = w.item;
+      if (first_item) share.continues = !starts, share.ends = ends;
+      first_item = false;
+    }
+    if (threadIdx.x == 128) parts.share[blockIdx.x] = share;
+    if (*abort_flag != 0 && lane == 0) atomicCAS(p.status, 0, kStatusEpilogueTimeout);
   }
-#pragma unroll
-  for (int i = 0; i < E; ++i)
-    p.out[((long long)row * p.heads + h) * D + lane * E + i] = __float2bfloat16(l > 0.f ? o[i] / l : 0.f);
+
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag != 0) {
+    // a wait gave up: let copies that are still in flight land before the CTA retires
+    const unsigned long long t0 = global_timer_ns();
+    while (global_timer_ns() - t0 < 2000000ull) __nanosleep(1000);
+    __syncthreads();
+  }
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, C::TMEM_COLS);
+  }
 }
 
 }  // namespace
@@ -596,15 +1086,38 @@ bool pages_tmap(CUtensorMap* map, const bf16* base, const PagedAttention& p, int
   return r == CUDA_SUCCESS;
 }
 
-// rows of the tile that takes the most rows a sequence can have here, 64 at most
-int tile_rows(const PagedAttention& p) {
-  const long long most = (long long)p.max_new * (p.heads / p.kv_heads);
-  return most <= 16 ? 16 : most <= 32 ? 32 : 64;
+// [tokens][heads][head_dim] of the queries; box = 64 columns of a query tile's heads and tokens
+bool queries_tmap(CUtensorMap* map, const PagedAttention& p, int head_dim, const Tiling& tl) {
+  EncodeFn fn = attn_encode_fn();
+  if (!fn) return false;
+  const cuuint64_t dims[3] = {(cuuint64_t)head_dim, (cuuint64_t)p.heads, (cuuint64_t)p.tokens};
+  const cuuint64_t strides[2] = {(cuuint64_t)(p.heads == 1 ? head_dim : p.q_head) * 2, (cuuint64_t)(p.tokens == 1 ? head_dim : p.q_token) * 2};
+  const cuuint32_t boxes[3] = {64, (cuuint32_t)tl.group, (cuuint32_t)(tl.tokens / tl.tiles)}, estr[3] = {1, 1, 1};
+  auto encode = [&] {
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<bf16*>(p.q), dims, strides, boxes, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult r = encode();
+  if (r == CUDA_ERROR_INVALID_CONTEXT && bind_primary_context()) r = encode();  // the first call of a thread
+  return r == CUDA_SUCCESS;
 }
-int rows_ctas() { return 2 * attn_grid(1 << 20); }
+
+// How a call is run.  Either kernel takes any rows; what a sequence typically has decides: twice the mean, or the most where the
+// caller knows less.
+struct Plan {
+  Tiling tl;
+  int ctas;
+  explicit Plan(const PagedAttention& p) {
+    const long long group = p.heads / p.kv_heads, typical = (2ll * p.tokens + p.seqs - 1) / p.seqs;
+    const long long rows = std::min<long long>(p.max_new, typical) * group;
+    tl = rows <= 64 ? Tiling(p, rows <= 16 ? 16 : rows <= 32 ? 32 : 64, 1, kRowsFixed) : Tiling(p, kBM, 2, kChunkFixed);
+    ctas = attn_grid(1 << 20) * (tl.tiles == 1 ? 2 : 1);
+  }
+  int rows() const { return tl.height * tl.tiles; }
+};
 
 template <typename C>
-cudaError_t rows_launch(const PagedAttention& p, const Parts& parts, int ctas, cudaStream_t stream) {
+cudaError_t rows_launch(const PagedAttention& p, const Parts& parts, const Plan& plan, cudaStream_t stream) {
   CUtensorMap tk, tv;
   const int box = std::min(kKeys, 1 << p.page_shift);
   if (!pages_tmap(&tk, p.k_pages, p, C::D, p.k_page, p.k_row, p.k_head, box) || !pages_tmap(&tv, p.v_pages, p, C::D, p.v_page, p.v_row, p.v_head, box))
@@ -614,41 +1127,58 @@ cudaError_t rows_launch(const PagedAttention& p, const Parts& parts, int ctas, c
     return cudaFuncSetAttribute(paged_rows_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
   });
   if (e != cudaSuccess) return e;
-  return launch_pdl(paged_rows_kernel<C>, dim3(ctas), dim3(kRowsThreads), C::SMEM, stream, 0, tk, tv, p, parts, FastDiv(p.heads / p.kv_heads));
+  return launch_pdl(paged_rows_kernel<C>, dim3(plan.ctas), dim3(kRowsThreads), C::SMEM, stream, 0, tk, tv, p, parts, plan.tl);
 }
 
 template <int D>
-cudaError_t attention_launch(const PagedAttention& p, void* work, int* launches, cudaStream_t stream) {
-  const int rows = tile_rows(p), ctas = rows_ctas();
-  Parts parts;
-  parts.rows = rows;
-  parts.acc = reinterpret_cast<float*>(work);
-  parts.ml = reinterpret_cast<float2*>(parts.acc + 2ll * ctas * rows * D);
-  parts.share = reinterpret_cast<Share*>(parts.ml + 2ll * ctas * rows);
-  cudaError_t e = rows == 16   ? rows_launch<Rows<D, 1>>(p, parts, ctas, stream)
-                  : rows == 32 ? rows_launch<Rows<D, 2>>(p, parts, ctas, stream)
-                               : rows_launch<Rows<D, 4>>(p, parts, ctas, stream);
+cudaError_t chunk_launch(const PagedAttention& p, const Parts& parts, const Plan& plan, cudaStream_t stream) {
+  using C = Chunk<D>;
+  CUtensorMap tq, tk, tv;
+  const int box = std::min(kBM, 1 << p.page_shift);
+  if (!queries_tmap(&tq, p, D, plan.tl) || !pages_tmap(&tk, p.k_pages, p, D, p.k_page, p.k_row, p.k_head, box) ||
+      !pages_tmap(&tv, p.v_pages, p, D, p.v_page, p.v_row, p.v_head, box))
+    return cudaErrorInvalidValue;
+  auto kernel = paged_chunk_kernel<D>;
+  static std::atomic<unsigned long long> granted{0};
+  const cudaError_t e = once_per_device(granted, [&] {
+    cudaFuncAttributes fa;
+    // the register shares of the kernel's warps add up to what it is launched with, or the larger one waits forever
+    if (cudaFuncGetAttributes(&fa, kernel) != cudaSuccess || fa.numRegs != 168) return cudaErrorInvalidConfiguration;
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+  });
   if (e != cudaSuccess) return e;
-  *launches = 2;
-  if ((long long)p.max_new * (p.heads / p.kv_heads) > rows) {
-    const long long warps = (long long)p.tokens * p.heads;
-    e = launch_pdl(paged_attention_kernel<D>, dim3((unsigned)((warps + 3) / 4)), dim3(128), 0, stream, 0, p, rows);
-    if (e != cudaSuccess) return e;
-    ++*launches;
-  }
-  return launch_pdl(paged_join_kernel<D>, dim3(ctas, rows / 16), dim3(256), 0, stream, 0, p, parts, ctas);
+  return launch_pdl(kernel, dim3(plan.ctas), dim3(kChunkThreads), C::SMEM, stream, 0, tq, tk, tv, p, parts, plan.tl);
+}
+
+template <int D>
+cudaError_t attention_launch(const PagedAttention& p, void* work, cudaStream_t stream) {
+  const Plan plan(p);
+  Parts parts;
+  parts.acc = reinterpret_cast<float*>(work);
+  parts.ml = reinterpret_cast<float2*>(parts.acc + 2ll * plan.ctas * plan.rows() * D);
+  parts.share = reinterpret_cast<Share*>(parts.ml + 2ll * plan.ctas * plan.rows());
+  const cudaError_t e = plan.rows() == 16   ? rows_launch<Rows<D, 1>>(p, parts, plan, stream)
+                        : plan.rows() == 32 ? rows_launch<Rows<D, 2>>(p, parts, plan, stream)
+                        : plan.rows() == 64 ? rows_launch<Rows<D, 4>>(p, parts, plan, stream)
+                                            : chunk_launch<D>(p, parts, plan, stream);
+  if (e != cudaSuccess) return e;
+  // of a tile's rows those that a sequence can have
+  const long long most = std::min<long long>(plan.rows(), (long long)p.max_new * (p.heads / p.kv_heads));
+  if (plan.tl.tiles == 1)
+    return launch_pdl(paged_join_kernel<D, 8>, dim3(plan.ctas, (unsigned)std::min<long long>(most, 16)), dim3(256), 0, stream, 0, p, parts, plan.tl);
+  return launch_pdl(paged_join_kernel<D, 1>, dim3(plan.ctas, 16), dim3(256), 0, stream, 0, p, parts, plan.tl);
 }
 
 }  // namespace
 
 long long paged_attention_workspace(const PagedAttention& p, int head_dim) {
-  const long long rows = tile_rows(p), ctas = rows_ctas();
-  return 2 * ctas * rows * (head_dim * sizeof(float) + sizeof(float2)) + ctas * sizeof(Share);
+  const Plan plan(p);
+  return 2ll * plan.ctas * plan.rows() * (head_dim * sizeof(float) + sizeof(float2)) + plan.ctas * sizeof(Share);
 }
 
-cudaError_t paged_attention_launch(const PagedAttention& p, int head_dim, void* work, int* launches, cudaStream_t stream) {
-  if (head_dim == 64) return attention_launch<64>(p, work, launches, stream);
-  if (head_dim == 128) return attention_launch<128>(p, work, launches, stream);
+cudaError_t paged_attention_launch(const PagedAttention& p, int head_dim, void* work, cudaStream_t stream) {
+  if (head_dim == 64) return attention_launch<64>(p, work, stream);
+  if (head_dim == 128) return attention_launch<128>(p, work, stream);
   return cudaErrorInvalidValue;
 }
 
