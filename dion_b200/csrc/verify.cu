@@ -11,10 +11,15 @@ namespace dion {
 
 namespace {
 
-constexpr int kVerifyThreads = 512, kVerifyWarps = kVerifyThreads / 32;
+constexpr int kVerifyThreads = 256, kVerifyWarps = kVerifyThreads / 32;
 constexpr int kVerifyCluster = 8;  // CTAs of a sequence
+constexpr int kVerifyGroups = 64;  // parts of a warp's tokens that the search tells apart
 
-__device__ __forceinline__ double usable(double w) { return w > 0.0 && w < INFINITY ? w : 0.0; }
+// t - q in 64 bits where that is positive and finite, else zero
+__device__ __forceinline__ double weight(float t, float q) {
+  const double d = (double)t - (double)q;
+  return t > q && d < INFINITY ? d : 0.0;
+}
 
 // the value of `v` in CTA `rank` of the cluster
 __device__ __forceinline__ double remote(const double* v, int rank) {
@@ -32,10 +37,10 @@ __device__ __forceinline__ double remote(const double* v, int rank) {
 // 1e-16 of the whole, the border that a draw has to hit to tell them apart.
 //
 // A warp takes consecutive tokens, 32 x 4 at a time (16 bytes a lane where the rows allow), so that the search goes down from the
-// CTA's sum over the warps' to one warp, which alone goes through its tokens again.
+// CTA's sum over a warp's to one warp's tokens, which all warps of that CTA go through again, and to one group of these.
 template <int V>
 __global__ void __cluster_dims__(kVerifyCluster, 1, 1) __launch_bounds__(kVerifyThreads) verify_drafts_kernel(const VerifyDrafts p) {
-  __shared__ double warp_sum[2][kVerifyWarps + 1];  // of the differences and of the row itself; the CTA's in the end
+  __shared__ double warp_sum[kVerifyWarps + 1], group_sum[kVerifyGroups];  // the warps' and the CTA's
   pdl_trigger();
   pdl_wait();
   const int b = blockIdx.x / kVerifyCluster, rank = blockIdx.x % kVerifyCluster, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -69,117 +74,131 @@ __global__ void __cluster_dims__(kVerifyCluster, 1, 1) __launch_bounds__(kVerify
   const bool all = a == p.drafts;
   const float* row = p.target + b * p.target_seq + a * p.target_row;
   const float* minus = p.draft && !all ? p.draft + b * p.draft_seq + a * p.draft_row : nullptr;
-  const long long certain = !p.draft && !all ? x : -1;  // the draft's only token
+  int certain = !p.draft && !all && x < p.vocab ? (int)x : -1;  // the draft's only token
 
-  // V tokens of a lane: the differences and the row's own values
-  auto weights = [&](int i, double (&d)[V], double (&w)[V]) {
-    float t[V], q[V];
-    if constexpr (V == 4) {
-      const float4 r4 = i < p.vocab ? *reinterpret_cast<const float4*>(row + i) : make_float4(0.f, 0.f, 0.f, 0.f);
-      const float4 q4 = minus && i < p.vocab ? *reinterpret_cast<const float4*>(minus + i) : make_float4(0.f, 0.f, 0.f, 0.f);
-      t[0] = r4.x, t[1] = r4.y, t[2] = r4.z, t[3] = r4.w;
-      q[0] = q4.x, q[1] = q4.y, q[2] = q4.z, q[3] = q4.w;
-    } else {
-      t[0] = i < p.vocab ? row[i] : 0.f;
-      q[0] = minus && i < p.vocab ? minus[i] : 0.f;
-    }
+  // V tokens of a lane from i on, all at once or none
+  auto load = [&](const float* from, int i, float (&t)[V]) {
 #pragma unroll
-    for (int k = 0; k < V; ++k) {
-      w[k] = usable(t[k]);
-      d[k] = usable((double)t[k] - (i + k == certain ? 1.0 : (double)q[k]));
+    for (int k = 0; k < V; ++k) t[k] = 0.f;
+    if (!from || i >= p.vocab) return;
+    if constexpr (V == 4) {
+      const float4 v = *reinterpret_cast<const float4*>(from + i);
+      t[0] = v.x, t[1] = v.y, t[2] = v.z, t[3] = v.w;
+    } else {
+      t[0] = from[i];
     }
   };
   // tokens of this warp: `per` rounds of 32 * V
   constexpr int round = 32 * V, everybody = kVerifyCluster * kVerifyWarps * round;
   const int per = (int)(((long long)p.vocab + everybody - 1) / everybody);
-  const long long begin = ((long long)rank * kVerifyWarps + warp) * per * round;
-  double left = 0.0, whole = 0.0;
-#pragma unroll 4
-  for (int r = 0; r < per; ++r) {
-    const long long i = begin + r * round + lane * V;
-    if (i < p.vocab) {
-      double d[V], w[V];
-      weights((int)i, d, w);
+  const int begin = (rank * kVerifyWarps + warp) * per * round;  // the bindings keep the vocabulary so far below 2^31
+  // of rounds first .. last of the tokens from `from` on, in all lanes
+  auto sum_of = [&](int from, int first, int last) {
+    double sum = 0.0;
+    constexpr int AHEAD = 16 / V;  // rounds whose loads are under way at once
+    for (int r = first; r < last; r += AHEAD) {
+      float t[AHEAD][V], q[AHEAD][V];
+      const int i = from + r * round + lane * V;
 #pragma unroll
-      for (int k = 0; k < V; ++k) left += d[k], whole += w[k];
+      for (int j = 0; j < AHEAD; ++j) {
+        load(r + j < last ? row : nullptr, i + j * round, t[j]);
+        load(r + j < last ? minus : nullptr, i + j * round, q[j]);
+      }
+      const int c = certain - i;
+      if (certain >= 0 && c >= 0 && c < AHEAD * round) {
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j)
+#pragma unroll
+          for (int k = 0; k < V; ++k)
+            if (c == j * round + k) q[j][k] = 1.f;
+      }
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j)
+#pragma unroll
+        for (int k = 0; k < V; ++k) sum += weight(t[j][k], q[j][k]);
     }
-  }
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    left += __shfl_xor_sync(0xffffffffu, left, o);
-    whole += __shfl_xor_sync(0xffffffffu, whole, o);
-  }
-  if (lane == 0) warp_sum[0][warp] = left, warp_sum[1][warp] = whole;
-  __syncthreads();
-  if (threadIdx.x < 2) {
-    double s = 0.0;
-    for (int i = 0; i < kVerifyWarps; ++i) s += warp_sum[threadIdx.x][i];
-    warp_sum[threadIdx.x][kVerifyWarps] = s;
-  }
-  cluster_sync_all();
-  // which distribution, its sum, and what lies before this CTA
-  int which = all ? 1 : 0;
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    return sum;
+  };
   double total, before;
-  for (;; which = 1) {
-    const double mine = lane < kVerifyCluster ? remote(&warp_sum[which][kVerifyWarps], lane) : 0.0;
+  for (;;) {
+    const double sum = sum_of(begin, 0, per);
+    if (lane == 0) warp_sum[warp] = sum;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      double s = 0.0;
+      for (int i = 0; i < kVerifyWarps; ++i) s += warp_sum[i];
+      warp_sum[kVerifyWarps] = s;
+    }
+    cluster_sync_all();
+    const double mine = lane < kVerifyCluster ? remote(&warp_sum[kVerifyWarps], lane) : 0.0;
     total = before = 0.0;
     for (int i = 0; i < kVerifyCluster; ++i) {
       const double s = __shfl_sync(0xffffffffu, mine, i);
       if (i < rank) before += s;
       total += s;
     }
-    if (total > 0.0 || which == 1) break;  // p - q leaves nothing: p itself
+    if (total > 0.0 || (!minus && certain < 0)) break;
+    minus = nullptr, certain = -1;  // p - q leaves nothing: p itself
+    cluster_sync_all();
   }
   // The token is the first whose running sum exceeds the border.  The sums before a CTA are added up in one order by all of them, and
-  // those before a warp by all warps of its CTA; each of the two takes what lies before the next one's start, the last warp the rest,
-  // so that exactly one warp looks, wherever roundings put the border.
+  // those before a warp's tokens and before a group of these by all warps of the CTA; each takes what lies before the next one's
+  // start, the last one the rest, so that exactly one is searched, wherever roundings put the border.
   const double border = (double)u[p.drafts] * total;
   if (rank == 0 && threadIdx.x == 0) {
     p.accepted[b] = a;
     if (!(total > 0.0) || !(border < total)) p.token[b] = total > 0.0 && border >= total ? p.vocab - 1 : 0;  // the latter: a uniform that is none
   }
-  const bool here = total > 0.0 && border < total && (rank == 0 || before <= border) &&
-                    (rank == kVerifyCluster - 1 || before + warp_sum[which][kVerifyWarps] > border);
-  for (int i = 0; i < warp; ++i) before += warp_sum[which][i];
-  if (here && (warp == 0 || before <= border) && (warp == kVerifyWarps - 1 || before + warp_sum[which][warp] > border)) {
-    double run = before;
-    bool found = false;
-    for (int r = 0; r < per && !found; ++r) {
-      const long long i = begin + r * round + lane * V;
-      double d[V], w[V], mine = 0.0;
-#pragma unroll
-      for (int k = 0; k < V; ++k) d[k] = w[k] = 0.0;
-      if (i < p.vocab) weights((int)i, d, w);
-#pragma unroll
-      for (int k = 0; k < V; ++k) mine += which ? w[k] : d[k];
-      double upto = mine;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const double t = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += t;
-      }
-      const unsigned over = __ballot_sync(0xffffffffu, mine > 0.0 && run + upto > border);
-      found = over != 0;
-      if (found && lane == __ffs(over) - 1) {
-        double s = run + upto - mine;
-        long long token = i;
-        for (int k = 0; k < V; ++k) {
-          const double wk = which ? w[k] : d[k];
-          s += wk;
-          if (wk > 0.0) token = i + k;
-          if (wk > 0.0 && s > border) break;
-        }
-        p.token[b] = token;
-      }
-      run += __shfl_sync(0xffffffffu, upto, 31);
+  if (total > 0.0 && border < total && (rank == 0 || before <= border) &&
+      (rank == kVerifyCluster - 1 || before + warp_sum[kVerifyWarps] > border)) {
+    int owner = 0;
+    for (; owner < kVerifyWarps - 1 && before + warp_sum[owner] <= border; ++owner) before += warp_sum[owner];
+    const int from = (rank * kVerifyWarps + owner) * per * round;
+    const int each = (per + kVerifyGroups - 1) / kVerifyGroups, groups = (per + each - 1) / each;  // rounds of a group
+    for (int g = warp; g < groups; g += kVerifyWarps) {
+      const double sum = sum_of(from, g * each, min(per, (g + 1) * each));
+      if (lane == 0) group_sum[g] = sum;
     }
-    if (!found && lane == 0) {  // roundings put the border behind the warp's last token: the last one before it that can be drawn
-      long long i = min(begin + (long long)per * round, (long long)p.vocab) - 1;
-      for (; i > 0; --i) {
-        const double q = minus ? (double)minus[i] : i == certain ? 1.0 : 0.0;
-        if (usable(which ? (double)row[i] : (double)row[i] - q) > 0.0) break;
+    __syncthreads();
+    if (warp == 0) {
+      int g = 0;
+      for (; g < groups - 1 && before + group_sum[g] <= border; ++g) before += group_sum[g];
+      bool found = false;
+      for (int r = g * each; r < min(per, (g + 1) * each) && !found; ++r) {
+        const int i = from + r * round + lane * V;
+        float t[V], q[V];
+        load(row, i, t);
+        load(minus, i, q);
+        double w[V], mine = 0.0;
+#pragma unroll
+        for (int k = 0; k < V; ++k) mine += w[k] = weight(t[k], i + k == certain ? 1.f : q[k]);
+        double upto = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const double v = __shfl_up_sync(0xffffffffu, upto, o);
+          if (lane >= o) upto += v;
+        }
+        const unsigned over = __ballot_sync(0xffffffffu, mine > 0.0 && before + upto > border);
+        found = over != 0;
+        if (found && lane == __ffs(over) - 1) {
+          double s = before + upto - mine;
+          int token = i;
+          for (int k = 0; k < V; ++k) {
+            s += w[k];
+            if (w[k] > 0.0) token = i + k;
+            if (w[k] > 0.0 && s > border) break;
+          }
+          p.token[b] = token;
+        }
+        before += __shfl_sync(0xffffffffu, upto, 31);
       }
-      p.token[b] = max(i, 0ll);
+      if (!found && lane == 0) {  // roundings put the border behind the group's last token: the last one that can be drawn up to there
+        int i = min(from + min(per, (g + 1) * each) * round, p.vocab) - 1;
+        while (i > 0 && !(weight(row[i], i == certain ? 1.f : minus ? minus[i] : 0.f) > 0.0)) --i;
+        p.token[b] = max(i, 0);
+      }
     }
   }
   cluster_sync_all();  // nobody reads another's shared memory after this
