@@ -313,10 +313,9 @@ struct PagedAppend {
   long long q_token, q_head, k_token, k_in_head, v_token, v_in_head;
   long long k_page, k_row, k_head, v_page, v_row, v_head, cos_row, sin_row, table_pitch, table_rows;
   int tokens, seqs, heads, kv_heads, page_shift, pages, max_pages;
-  int tokens_per_block;  // the launcher's
   float eps;             // negative: no norm
 };
-cudaError_t paged_append_launch(PagedAppend p, int head_dim, bool wide_tables, cudaStream_t stream);
+cudaError_t paged_append_launch(const PagedAppend& p, int head_dim, bool wide_tables, cudaStream_t stream);
 
 struct PagedAttention {
   const __nv_bfloat16 *q, *k_pages, *v_pages;

@@ -3,6 +3,7 @@
 //   y = (x1 c + x2 s, x2 c - x1 s),  y *= rsqrt(mean(y^2) + eps),   c, s: the tables' rows at lengths[b] + i
 #include <cuda_bf16.h>
 
+#include "attention.cuh"
 #include "kernels.h"
 #include "paged.cuh"
 #include "pdl.cuh"
@@ -13,57 +14,77 @@ namespace {
 
 typedef __nv_bfloat16 bf16;
 
-constexpr int kAppendThreads = 256, kAppendTokens = 64;  // threads of a block, most tokens of one
+constexpr int kAppendThreads = 256;  // of a block, at most
+// Tokens of a block, where there are many.  16384 tokens, 32 heads and 8 kv heads of 128 (us): 68.0 with 2, 68.5 with 4, 94 with 8;
+// 33 prompts of up to 900, 12 heads of 64, with the norm: 32.1, 32.7, 44
+constexpr int kAppendTokens = 2;
 
-__device__ __forceinline__ void unpack8(const uint4& q, float (&f)[8]) {
-  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&q);
+// eight values as four pairs of fp32
+__device__ __forceinline__ void unpack8(const uint4& q, f32x2 (&f)[4]) {
+  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) f[j] = pack2(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xffff0000u));
+}
+__device__ __forceinline__ uint4 pack8(const f32x2 (&f)[4]) {
+  uint32_t w[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const float2 t = __bfloat1622float2(h[j]);
-    f[2 * j] = t.x;
-    f[2 * j + 1] = t.y;
+    float a, b;
+    unpack2(f[j], a, b);
+    w[j] = pack_bf16x2(a, b);
   }
-}
-__device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
-  uint4 q;
-  __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&q);
-#pragma unroll
-  for (int j = 0; j < 4; ++j) h[j] = __floats2bfloat162_rn(f[2 * j], f[2 * j + 1]);
-  return q;
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, float (&f)[8]) {
+__device__ __forceinline__ void load8(const T* p, f32x2 (&f)[4]) {
   if constexpr (sizeof(T) == 4) {
     const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-    f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
+    f[0] = pack2(a.x, a.y), f[1] = pack2(a.z, a.w), f[2] = pack2(b.x, b.y), f[3] = pack2(b.z, b.w);
   } else {
     unpack8(*reinterpret_cast<const uint4*>(p), f);
   }
 }
 
-// HD / 16 lanes share a row (one head of one token): eight pairs each, 16 bytes from either half of the head.  A block takes
-// `tokens_per_block` tokens, looks up their pages first and then goes through their H + 2 Hkv rows.
-template <int HD, typename Table>
+// HD / 16 lanes share a row (one head of one token): eight pairs each, 16 bytes from either half of the head.  A block takes T tokens
+// and as many of their rows as it has threads for, every thread the same row of each token, so that its addresses move on by one
+// stride.  Bound by memory: all loads of a thread are under way before it looks up where the rows go, and two fp32 operations go in one
+// instruction, as with single ones the issue slots were half full.
+template <int HD, int T, typename Table>
 __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const PagedAppend p) {
   constexpr int HALF = HD / 2, LPR = HD / 16;
-  __shared__ long long k_at[kAppendTokens], v_at[kAppendTokens];  // of a token's rows in the pages; -1: it has none
-  __shared__ int position[kAppendTokens];
+  __shared__ long long k_at[T], v_at[T];  // of a token's rows in the pages; -1: it has none
+  __shared__ int position[T];
   pdl_trigger();
   pdl_wait();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int t0 = blockIdx.x * p.tokens_per_block, tokens = min(p.tokens_per_block, p.tokens - t0);
-  if (blockIdx.x == 0) {  // offsets start at zero, never fall and end within the tokens
+  const int lane = threadIdx.x & 31, col = (threadIdx.x % LPR) * 8;
+  const int t0 = (int)blockIdx.x * T, r = (int)(blockIdx.y * (blockDim.x / LPR) + threadIdx.x / LPR);
+  const bool of_q = r < p.heads, of_k = !of_q && r < p.heads + p.kv_heads, there = r < p.heads + 2 * p.kv_heads;
+  const int h = of_q ? r : of_k ? r - p.heads : r - p.heads - p.kv_heads;
+  uint4 lo[T], hi[T];
+  if (there) {
+    const long long step = of_q ? p.q_token : of_k ? p.k_token : p.v_token;
+    const bf16* src = (of_q ? p.q : of_k ? p.k : p.v) + t0 * step + h * (of_q ? p.q_head : of_k ? p.k_in_head : p.v_in_head) + col;
+#pragma unroll
+    for (int j = 0; j < T; ++j) {
+      if (T == 1 || t0 + j < p.tokens) {
+        lo[j] = *reinterpret_cast<const uint4*>(src);
+        hi[j] = *reinterpret_cast<const uint4*>(src + HALF);
+      }
+      src += step;
+    }
+  }
+  if (blockIdx.x == 0 && blockIdx.y == 0) {  // offsets start at zero, never fall and end within the tokens
     bool bad = threadIdx.x == 0 && (p.offsets[0] != 0 || p.offsets[p.seqs] > p.tokens);
-    for (int b = threadIdx.x; b < p.seqs; b += kAppendThreads) bad |= p.offsets[b] > p.offsets[b + 1];
+    for (int b = threadIdx.x; b < p.seqs; b += blockDim.x) bad |= p.offsets[b] > p.offsets[b + 1];
     if (bad) bad_argument(p.status);
   }
-  for (int i = warp; i < tokens; i += kAppendThreads / 32) {
-    const int row = t0 + i, b = sequence_of(p.offsets, p.seqs, row, lane);
+  for (int j = threadIdx.x / 32; j < T; j += blockDim.x / 32) {  // a warp per token
+    const int row = t0 + j, b = sequence_of(p.offsets, p.seqs, row, lane);
     if (lane == 0) {
       const int first = p.offsets[b], end = p.offsets[b + 1];
       long long ka = -1, va = -1;
       int pos = 0;
-      if (row >= first && row < end) {
+      if (row >= first && row < end && row < p.tokens) {
         const long long at = (long long)p.lengths[b] + ((long long)row - first), slot = at >> p.page_shift;
         int page = -1;
         if (p.lengths[b] >= 0 && at < p.table_rows && slot < p.max_pages) page = p.page_table[(long long)b * p.table_pitch + slot];
@@ -76,79 +97,74 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const Page
           bad_argument(p.status);
         }
       }
-      k_at[i] = ka, v_at[i] = va, position[i] = pos;
+      k_at[j] = ka, v_at[j] = va, position[j] = pos;
     }
   }
   __syncthreads();
-  const int rows = p.heads + 2 * p.kv_heads, units = rows * LPR;
-  const int total = (tokens * units + 31) / 32 * 32;  // whole warps, for the shuffles
-  for (int u = threadIdx.x; u < total; u += kAppendThreads) {
-    const bool live = u < tokens * units;
-    const int i = live ? u / units : 0, r = live ? (u - i * units) / LPR : 0, col = (u % LPR) * 8;
-    const long long token = t0 + i;
-    const long long to_k = k_at[i];
-    const bf16* src;
-    bf16* dst;
-    if (r < p.heads) {
-      src = p.q + token * p.q_token + r * p.q_head;
-      dst = p.q_out + (token * p.heads + r) * HD;
-    } else if (r < p.heads + p.kv_heads) {
-      const int h = r - p.heads;
-      src = p.k + token * p.k_token + h * p.k_in_head;
-      dst = p.k_pages + to_k + h * p.k_head;
-    } else {
-      const int h = r - p.heads - p.kv_heads;
-      src = p.v + token * p.v_token + h * p.v_in_head;
-      dst = p.v_pages + v_at[i] + h * p.v_head;
-    }
-    uint4 a = *reinterpret_cast<const uint4*>(src + col), b = *reinterpret_cast<const uint4*>(src + col + HALF);
-    const bool turn = r < p.heads + p.kv_heads;
-    float x1[8], x2[8], c[8], s[8], y1[8], y2[8], ss = 0.f;
-    unpack8(a, x1);
-    unpack8(b, x2);
-    const long long at = (long long)position[i] * p.cos_row + col, sat = (long long)position[i] * p.sin_row + col;
-    load8(reinterpret_cast<const Table*>(p.cos) + at, c);
-    load8(reinterpret_cast<const Table*>(p.sin) + sat, s);
+  if (!there) return;
+  const unsigned row_lanes = ((1u << LPR) - 1) << (lane & ~(LPR - 1));  // the lanes of this row: all or none of them get here
+  bf16* to = (of_q ? p.q_out + ((long long)t0 * p.heads + h) * HD : of_k ? p.k_pages + h * p.k_head : p.v_pages + h * p.v_head) + col;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      y1[j] = x1[j] * c[j] + x2[j] * s[j];
-      y2[j] = x2[j] * c[j] - x1[j] * s[j];
-      ss += y1[j] * y1[j] + y2[j] * y2[j];
-    }
-    if (p.eps >= 0.f) {
+  for (int j = 0; j < T; ++j) {
+    if (T > 1 && t0 + j >= p.tokens) break;
+    const long long at = of_k ? k_at[j] : v_at[j];
+    uint4 a = lo[j], b = hi[j];
+    if (of_q || of_k) {
+      f32x2 x1[4], x2[4], c[4], s[4];
+      unpack8(a, x1);
+      unpack8(b, x2);
+      load8(reinterpret_cast<const Table*>(p.cos) + (long long)position[j] * p.cos_row + col, c);
+      load8(reinterpret_cast<const Table*>(p.sin) + (long long)position[j] * p.sin_row + col, s);
+      float ss = 0.f;
 #pragma unroll
-      for (int o = LPR / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      const float f = rsqrtf(ss / (float)HD + p.eps);
+      for (int e = 0; e < 4; ++e) {  // the operations of the training kernels in their order, and so their bits
+        const f32x2 minus_s = s[e] ^ 0x8000000080000000ull;
+        const f32x2 y1 = fma2(x1[e], c[e], mul2(x2[e], s[e])), y2 = fma2(x2[e], c[e], mul2(x1[e], minus_s));
+        x1[e] = y1, x2[e] = y2;
+        float s0, s1;
+        unpack2(fma2(y1, y1, mul2(y2, y2)), s0, s1);
+        ss += s0;
+        ss += s1;
+      }
+      if (p.eps >= 0.f) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) y1[j] *= f, y2[j] *= f;
+        for (int o = LPR / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(row_lanes, ss, o);
+        const float f = rsqrtf(ss / (float)HD + p.eps);
+        const f32x2 f2 = pack2(f, f);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x1[e] = mul2(x1[e], f2), x2[e] = mul2(x2[e], f2);
+      }
+      a = pack8(x1);
+      b = pack8(x2);
     }
-    if (turn) a = pack8(y1), b = pack8(y2);
-    if (to_k < 0) {  // nobody's row: its query becomes zero, nothing goes to the pages
-      a = b = make_uint4(0, 0, 0, 0);
-      if (r >= p.heads) continue;
-    }
-    if (live) {
-      *reinterpret_cast<uint4*>(dst + col) = a;
-      *reinterpret_cast<uint4*>(dst + col + HALF) = b;
+    if (at < 0) a = b = make_uint4(0, 0, 0, 0);  // nobody's row: its query becomes zero, nothing goes to the pages
+    if (of_q || at >= 0) {
+      bf16* dst = of_q ? to + (long long)j * p.heads * HD : to + at;
+      *reinterpret_cast<uint4*>(dst) = a;
+      *reinterpret_cast<uint4*>(dst + HALF) = b;
     }
   }
 }
 
+template <int HD, typename Table>
+cudaError_t append_launch(const PagedAppend& p, cudaStream_t stream) {
+  constexpr int step = 32 / (HD / 16);  // rows of a warp
+  const int rows = p.heads + 2 * p.kv_heads, most = kAppendThreads / 32 * step;
+  const int parts = (rows + most - 1) / most, each = ((rows + parts - 1) / parts + step - 1) / step * step;  // blocks of a token, rows of one
+  if (parts > 65535) return cudaErrorInvalidValue;
+  const dim3 block(each * (HD / 16));
+  // one token a block while that leaves SMs without a block
+  if ((long long)p.tokens * parts <= 4ll * 148 * kAppendTokens)
+    return launch_pdl(paged_append_kernel<HD, 1, Table>, dim3(p.tokens, parts), block, 0, stream, 0, p);
+  return launch_pdl(paged_append_kernel<HD, kAppendTokens, Table>, dim3((p.tokens + kAppendTokens - 1) / kAppendTokens, parts), block, 0, stream, 0, p);
+}
+
 }  // namespace
 
-cudaError_t paged_append_launch(PagedAppend p, int head_dim, bool wide_tables, cudaStream_t stream) {
+cudaError_t paged_append_launch(const PagedAppend& p, int head_dim, bool wide_tables, cudaStream_t stream) {
   if (p.tokens <= 0) return cudaSuccess;
-  const int units = (p.heads + 2 * p.kv_heads) * (head_dim / 16);
-  // two rounds of a block's threads
-  p.tokens_per_block = units >= 2 * kAppendThreads ? 1 : 2 * kAppendThreads / units;
-  if (p.tokens_per_block > kAppendTokens) p.tokens_per_block = kAppendTokens;
-  const dim3 grid((p.tokens + p.tokens_per_block - 1) / p.tokens_per_block), block(kAppendThreads);
-  if (head_dim == 64)
-    return wide_tables ? launch_pdl(paged_append_kernel<64, float>, grid, block, 0, stream, 0, p)
-                       : launch_pdl(paged_append_kernel<64, bf16>, grid, block, 0, stream, 0, p);
-  if (head_dim == 128)
-    return wide_tables ? launch_pdl(paged_append_kernel<128, float>, grid, block, 0, stream, 0, p)
-                       : launch_pdl(paged_append_kernel<128, bf16>, grid, block, 0, stream, 0, p);
+  if (head_dim == 64) return wide_tables ? append_launch<64, float>(p, stream) : append_launch<64, bf16>(p, stream);
+  if (head_dim == 128) return wide_tables ? append_launch<128, float>(p, stream) : append_launch<128, bf16>(p, stream);
   return cudaErrorInvalidValue;
 }
 
