@@ -20,6 +20,7 @@ from torch.distributed.tensor import DTensor, Replicate, Shard
 
 from ..ops import nn as K
 from ..parallel import tp as TP
+from .generation import CacheStep, PagedCache, generate_cached, generate_drafted
 
 
 @dataclass
@@ -109,6 +110,13 @@ class CausalSelfAttention(nn.Module):
             return residual + TP.row_parallel_linear(y, _local(self.c_proj.weight), group)
         return K.linear(y, _local(self.c_proj.weight), residual=residual)
 
+    def forward_cached(self, h: torch.Tensor, residual: torch.Tensor, step: CacheStep, layer: int) -> torch.Tensor:
+        """The same for the new tokens of a cache's sequences, [1, tokens, C]."""
+        q, k, v = (t.view(h.shape[1], -1, self.head_dim) for t in K.linear_fanout(
+            h, _local(self.c_q.weight), _local(self.c_k.weight), _local(self.c_v.weight)))
+        y = step.attend(layer, q, k, v, *self.rotary.tables(step.cache.max_len, h.device), norm_eps=K.RMS_EPS)
+        return K.linear(y.view(1, h.shape[1], -1), _local(self.c_proj.weight), residual=residual)
+
 
 class MLP(nn.Module):
     def __init__(self, config: GPTConfig):
@@ -162,7 +170,12 @@ class Block(nn.Module):
         return torch.ops.dion_b200.gpt_block_fwd(x, *shadows, cos, sin, attn.head_dim, K.RMS_EPS, on_kernels,
                                                  K.runtime.status_tensor(x.device))
 
-    def forward(self, x: torch.Tensor, bt=None) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, bt=None, step: Optional[CacheStep] = None, layer: int = 0) -> torch.Tensor:
+        if step is not None:
+            x, h = K.norm_branch(x)
+            x = self.attn.forward_cached(h, x, step, layer)
+            x, h = K.norm_branch(x)
+            return self.mlp(h, x)
         if bt is None and not torch.is_grad_enabled():
             y = self._forward_native(x)
             if y is not None:
@@ -172,6 +185,15 @@ class Block(nn.Module):
         x, h = K.norm_branch(x)
         x = self.mlp(h, x, bt)
         return x
+
+
+def _refuse_drafts_of_shards(*models: nn.Module) -> None:
+    """The ranks that hold a sharded model have to make the same passes, and how many drafts stand is a matter of each rank."""
+    a, b = (m.config.vocab_size for m in models)
+    if a != b:
+        raise ValueError(f"a draft of a vocabulary of {b} tokens for one of {a}")
+    if any(isinstance(p, DTensor) for m in models for p in m.parameters()):
+        raise ValueError("drafts are for models whose weights are whole on every rank")
 
 
 class GPT(nn.Module):
@@ -210,7 +232,9 @@ class GPT(nn.Module):
         return torch.bfloat16 if torch.device(device).type == "cuda" else self.lm_head.weight.dtype
 
     # -- forward
-    def forward(self, idx, targets=None, return_logits=False):
+    def forward(self, idx, targets=None, return_logits=False, cache: Optional[CacheStep] = None):
+        if cache is not None:
+            return self._forward_cached(idx, cache)
         bt = self._sequence_parallel_shape(idx)
         x = self._forward_emb(idx, bt)
         return self._forward(x, targets, return_logits, bt)
@@ -265,6 +289,23 @@ class GPT(nn.Module):
             logits = K.linear(x, _local(w))
         return logits.float()
 
+    def _forward_cached(self, tokens: torch.Tensor, step: CacheStep) -> torch.Tensor:
+        """fp32 logits [rows that the step wants, vocabulary] of the new tokens of a cache's sequences."""
+        if _tp_group(self.lm_head.weight)[0] is not None:
+            raise RuntimeError("a cache of keys and values goes with whole weights, not with tensor-parallel ones")
+        x = K.embedding(tokens, _local(self.transformer.wte.weight), self._act_dtype(tokens.device))[None]
+        for i, block in enumerate(self.transformer.h):
+            x = block(x, step=step, layer=i)
+        return K.linear(K.rms_norm(step.wanted(x[0])[None]), _local(self.lm_head.weight))[0].float()
+
+    def new_cache(self, sequences: int, max_len: Optional[int] = None, page_size: int = 64, pages: Optional[int] = None) -> PagedCache:
+        """An empty cache for `sequences` texts of up to `max_len` tokens (the model's by default)."""
+        c, w = self.config, self.lm_head.weight
+        max_len = c.sequence_len if max_len is None else max_len
+        if max_len > c.sequence_len:
+            raise ValueError(f"a cache for {max_len} tokens, the model takes {c.sequence_len}")
+        return PagedCache(c.n_layer, c.n_head, c.n_embd // c.n_head, sequences, max_len, page_size, pages, self._act_dtype(w.device), w.device)
+
     def compile(self):  # noqa: A003 - API parity with the reference (models/gpt_model.py:195-200)
         """The reference compiles the forward with torch.compile; here the forward already runs
         on hand-written kernels, so this is a no-op kept for API compatibility."""
@@ -276,8 +317,20 @@ class GPT(nn.Module):
 
     @torch.no_grad()
     def generate(self, input_ids: torch.LongTensor, max_new_tokens: int, temperature: float = 1.0,
-                 top_k: Optional[int] = None) -> torch.LongTensor:
-        """Sample `max_new_tokens` tokens, feeding at most `sequence_len` tokens of context."""
+                 top_k: Optional[int] = None, use_cache: bool = False, draft_model: Optional["GPT"] = None,
+                 draft_tokens: int = 4) -> torch.LongTensor:
+        """Sample `max_new_tokens` tokens, feeding at most `sequence_len` tokens of context.
+
+        With `use_cache` the keys and values of earlier tokens are kept in a paged cache and every pass sees the new token alone;
+        prompt and new tokens have to fit `sequence_len` then.  With `draft_model`, a smaller model of the same vocabulary, that
+        one proposes `draft_tokens` tokens at a time and this one checks them in a single pass over its cache; the
+        tokens are distributed as without."""
+        if draft_model is not None:
+            _refuse_drafts_of_shards(self, draft_model)
+            return generate_drafted(self, self.config.sequence_len, draft_model, draft_model.config.sequence_len, draft_tokens,
+                                    input_ids, max_new_tokens, temperature, top_k)
+        if use_cache:
+            return generate_cached(self, self.config.sequence_len, input_ids, max_new_tokens, temperature, top_k)
         idx = input_ids
         for _ in range(max_new_tokens):
             ctx = idx if idx.size(1) <= self.config.sequence_len else idx[:, -self.config.sequence_len:]

@@ -20,6 +20,8 @@ from torch.distributed.device_mesh import DeviceMesh
 from torch.distributed.tensor import Shard
 
 from ..ops import nn as K
+from .generation import CacheStep, PagedCache, generate_cached, generate_drafted
+from .gpt import _refuse_drafts_of_shards
 
 
 @dataclass
@@ -77,6 +79,12 @@ class LlamaAttention(nn.Module):
         y = K.causal_attention(q, k, v)
         return K.linear(y, self.wo.weight, residual=residual)
 
+    def forward_cached(self, h: torch.Tensor, residual: torch.Tensor, step: CacheStep, layer: int) -> torch.Tensor:
+        """The same for the new tokens of a cache's sequences, [1, tokens, C]."""
+        q, k, v = (K.linear(h, w.weight).view(h.shape[1], -1, self.head_dim) for w in (self.wq, self.wk, self.wv))
+        y = step.attend(layer, q, k, v, *self._rope(step.cache.max_len, h.device))
+        return K.linear(y.view(1, h.shape[1], -1), self.wo.weight, residual=residual)
+
 
 class LlamaMLP(nn.Module):
     def __init__(self, cfg: LlamaConfig):
@@ -99,8 +107,11 @@ class LlamaBlock(nn.Module):
         self.ffn_norm = RMSNormGain(cfg.n_embd, cfg.norm_eps)
         self.feed_forward = LlamaMLP(cfg)
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
-        x = self.attention(self.attention_norm(x), x)
+    def forward(self, x: torch.Tensor, step: Optional[CacheStep] = None, layer: int = 0) -> torch.Tensor:
+        if step is not None:
+            x = self.attention.forward_cached(self.attention_norm(x), x, step, layer)
+        else:
+            x = self.attention(self.attention_norm(x), x)
         x = self.feed_forward(self.ffn_norm(x), x)
         return x
 
@@ -123,7 +134,10 @@ class Llama(nn.Module):
             elif isinstance(m, RMSNormGain):
                 nn.init.ones_(m.weight)
 
-    def forward(self, idx: torch.Tensor, targets: Optional[torch.Tensor] = None, return_logits: bool = False):
+    def forward(self, idx: torch.Tensor, targets: Optional[torch.Tensor] = None, return_logits: bool = False,
+                cache: Optional[CacheStep] = None):
+        if cache is not None:
+            return self._forward_cached(idx, cache)
         dtype = torch.bfloat16 if idx.is_cuda else self.output.weight.dtype
         x = K.embedding(idx, self.tok_embeddings.weight, dtype)
         for layer in self.layers:
@@ -136,6 +150,34 @@ class Llama(nn.Module):
                 return None
             x = x[:, [-1], :]
         return K.linear(x, self.output.weight).float()
+
+    def _forward_cached(self, tokens: torch.Tensor, step: CacheStep) -> torch.Tensor:
+        """fp32 logits [rows that the step wants, vocabulary] of the new tokens of a cache's sequences."""
+        dtype = torch.bfloat16 if tokens.is_cuda else self.output.weight.dtype
+        x = K.embedding(tokens, self.tok_embeddings.weight, dtype)[None]
+        for i, layer in enumerate(self.layers):
+            x = layer(x, step=step, layer=i)
+        return K.linear(self.norm(step.wanted(x[0])[None]), self.output.weight)[0].float()
+
+    def new_cache(self, sequences: int, max_len: Optional[int] = None, page_size: int = 64, pages: Optional[int] = None) -> PagedCache:
+        """An empty cache for `sequences` texts of up to `max_len` tokens (the model's by default)."""
+        c, w = self.config, self.output.weight
+        max_len = c.sequence_len if max_len is None else max_len
+        if max_len > c.sequence_len:
+            raise ValueError(f"a cache for {max_len} tokens, the model takes {c.sequence_len}")
+        dtype = torch.bfloat16 if w.is_cuda else w.dtype
+        return PagedCache(c.n_layer, c.n_kv_head, c.n_embd // c.n_head, sequences, max_len, page_size, pages, dtype, w.device)
+
+    @torch.no_grad()
+    def generate(self, input_ids: torch.LongTensor, max_new_tokens: int, temperature: float = 1.0, top_k: Optional[int] = None,
+                 draft_model: Optional["Llama"] = None, draft_tokens: int = 4) -> torch.LongTensor:
+        """Sample `max_new_tokens` tokens over a paged cache; prompt and new tokens have to fit `sequence_len`.  `draft_model`
+        and `draft_tokens` as for ``GPT.generate``."""
+        if draft_model is not None:
+            _refuse_drafts_of_shards(self, draft_model)
+            return generate_drafted(self, self.config.sequence_len, draft_model, draft_model.config.sequence_len, draft_tokens,
+                                    input_ids, max_new_tokens, temperature, top_k)
+        return generate_cached(self, self.config.sequence_len, input_ids, max_new_tokens, temperature, top_k)
 
 
 def make_llama_param_groups(model: Llama, scalar_opt: str = "adamw", lr: float = 0.01) -> List[dict]:

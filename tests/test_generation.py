@@ -1,0 +1,200 @@
+"""Sampling over a paged cache: the cache's bookkeeping, cached passes against whole ones, and drafts."""
+import pytest
+import torch
+
+from dion_b200 import ops
+from dion_b200.models import GPT, GPTConfig, Llama, LlamaConfig, PagedCache
+from dion_b200.ops import nn as N
+
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+
+
+def _gpt(layers=2, width=64, heads=4, seq=64, vocab=97, device="cpu"):
+    m = GPT(GPTConfig(sequence_len=seq, vocab_size=vocab, n_layer=layers, n_head=heads, n_embd=width)).to(device)
+    m.init_weights()
+    return m
+
+
+def _llama(layers=2, width=64, heads=4, kv_heads=2, seq=64, vocab=97, device="cpu"):
+    m = Llama(LlamaConfig(sequence_len=seq, vocab_size=vocab, n_layer=layers, n_head=heads, n_kv_head=kv_heads, n_embd=width, ffn_dim=2 * width)).to(device)
+    m.init_weights(std=0.2)
+    return m
+
+
+def _whole_logits(m, idx):
+    """Logits of every position by the pass that training makes."""
+    return m(idx, idx, return_logits=True)
+
+
+# --------------------------------------------------------------------------- the cache
+
+def test_cache_takes_pages_as_sequences_grow_and_gives_them_back():
+    c = PagedCache(2, 3, 8, sequences=3, max_len=100, page_size=16, pages=9, dtype=torch.float32, device="cpu")
+    s = c.step([20, 0, 16])
+    assert c.lengths == [20, 0, 16] and c.free_pages == 6
+    assert s.offsets.tolist() == [0, 20, 20, 36] and s.lengths.tolist() == [0, 0, 0] and s.max_new == 20 and s.rows == [19, 35]
+    s = c.step([1, 5, 1], all_rows=True)
+    assert s.lengths.tolist() == [20, 0, 16] and s.rows is None and c.free_pages == 4
+    used = [c._table[b, :n].tolist() for b, n in enumerate((2, 1, 2))]
+    assert len({p for u in used for p in u}) == 5
+    with pytest.raises(RuntimeError, match="free pages"):
+        c.step([60, 60, 0])
+    with pytest.raises(ValueError):
+        c.step([80, 0, 0])
+    with pytest.raises(ValueError):
+        c.step([1, 1])
+    with pytest.raises(ValueError):
+        c.step([1, -1, 0])
+    assert c.lengths == [21, 5, 17] and c.free_pages == 4  # a refused step changes nothing
+    with pytest.raises(ValueError):
+        c.cut([22, 0, 0])
+    c.cut([16, 0, 17])
+    assert c.free_pages == 6 and c.lengths == [16, 0, 17]
+    s = c.step([1, 33, 0])
+    assert c.free_pages == 2 and len({p for b, n in enumerate((2, 3, 2)) for p in s.page_table[b, :n].tolist()}) == 7
+    for bad in (dict(page_size=24), dict(page_size=8), dict(max_len=0), dict(sequences=0)):
+        with pytest.raises(ValueError):
+            PagedCache(**{**dict(layers=1, kv_heads=1, head_dim=8, sequences=1, max_len=10, device="cpu"), **bad})
+
+
+def test_a_step_taken_before_keeps_its_table():
+    c = PagedCache(1, 1, 8, sequences=2, max_len=64, page_size=16, dtype=torch.float32, device="cpu")
+    s = c.step([16, 16])
+    before = s.page_table.clone()
+    c.step([16, 16])
+    assert torch.equal(s.page_table, before) and s.lengths.tolist() == [0, 0]
+
+
+# --------------------------------------------------------------------------- passes over the cache
+
+@pytest.mark.parametrize("make", [_gpt, _llama])
+def test_cached_passes_give_the_logits_of_whole_ones(make):
+    """Chunk by chunk with ragged counts, in 64 bits but for the norms and the rotation of whole passes, which take 32: at most ten
+    roundings a layer, 21 with the head, each by at most a half step, on either side, as norms."""
+    torch.manual_seed(3)
+    m = make().double()
+    with torch.no_grad():
+        idx = torch.randint(0, 97, (3, 40))
+        want = _whole_logits(m, idx).double()
+        cache = m.new_cache(3, page_size=16)
+        done = [0, 0, 0]
+        for counts in ([5, 1, 0], [1, 0, 17], [20, 30, 1], [0, 1, 1], [14, 8, 21]):
+            tokens = torch.cat([idx[b, done[b]:done[b] + n] for b, n in enumerate(counts)])
+            got = m(tokens, cache=cache.step(counts, all_rows=True)).double()
+            at = 0
+            for b, n in enumerate(counts):
+                w = want[b, done[b]:done[b] + n]
+                assert (got[at:at + n] - w).norm() <= 2 * 21 * 2.0 ** -24 * w.norm()
+                at += n
+                done[b] += n
+        assert done == cache.lengths == [40, 40, 40]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("make,kw", [(_gpt, dict(width=256, heads=4)), (_gpt, dict(width=256, heads=2)), (_llama, dict(width=256, heads=4, kv_heads=2))])
+def test_cached_passes_on_the_kernels(make, kw):
+    """bf16 activations are rounded some ten times a layer on either way, each time by at most a half step: two layers and
+    the head are within 21 half steps of the exact, and of one another within twice that, as norms."""
+    torch.manual_seed(4)
+    m = make(seq=512, device="cuda", **kw)
+    with torch.no_grad():
+        idx = torch.randint(0, 97, (3, 400), device="cuda")
+        want = _whole_logits(m, idx)
+        cache = m.new_cache(3)
+        done = [0, 0, 0]
+        launches = ops.launch_count()
+        for counts in ([300, 1, 64], [1, 1, 0], [5, 300, 5], [1, 0, 200], [93, 98, 131]):
+            tokens = torch.cat([idx[b, done[b]:done[b] + n] for b, n in enumerate(counts)])
+            got = m(tokens, cache=cache.step(counts, all_rows=True))
+            at = 0
+            for b, n in enumerate(counts):
+                if n:
+                    w = want[b, done[b]:done[b] + n]
+                    assert (got[at:at + n] - w).norm() <= 2 * 21 * 2.0 ** -8 * w.norm()
+                at += n
+                done[b] += n
+        ops.check_status()
+        assert ops.launch_count() > launches and done == [400, 400, 400]
+
+
+# --------------------------------------------------------------------------- sampling
+
+def test_cached_sampling_draws_the_same_tokens():
+    torch.manual_seed(5)
+    m = _gpt()
+    idx = torch.randint(0, 97, (3, 7))
+    for kw in (dict(), dict(top_k=5), dict(temperature=0.5, top_k=1000)):
+        torch.manual_seed(9)
+        want = m.generate(idx, 20, **kw)
+        torch.manual_seed(9)
+        assert torch.equal(m.generate(idx, 20, use_cache=True, **kw), want)
+    assert torch.equal(m.generate(idx, 58, top_k=1, use_cache=True), m.generate(idx, 58, top_k=1))  # to the last position
+    assert torch.equal(m.generate(idx, 0, use_cache=True), idx)
+    with pytest.raises(ValueError, match="do not fit"):
+        m.generate(idx, 59, use_cache=True)
+    with pytest.raises(ValueError):
+        m.generate(idx[:, :0], 3, use_cache=True)
+
+
+def _greedy(m, idx, n):
+    for _ in range(n):
+        idx = torch.cat([idx, m(idx, return_logits=True)[:, -1].argmax(-1, keepdim=True)], 1)
+    return idx
+
+
+@pytest.mark.parametrize("make", [_gpt, _llama])
+@pytest.mark.parametrize("prompt", [1, 6])
+def test_greedy_tokens_do_not_depend_on_the_draft(make, prompt):
+    """The most likely token every time, whatever a draft proposes: itself (always right), a smaller model (mostly wrong)."""
+    torch.manual_seed(6)
+    m, small = make(), make(layers=1, width=32, heads=2, **(dict(kv_heads=1) if make is _llama else {}))
+    idx = torch.randint(0, 97, (4, prompt))
+    want = _greedy(m, idx, 25)
+    assert torch.equal(m.generate(idx, 25, top_k=1, **({} if make is _llama else dict(use_cache=True))), want)
+    for draft in (m, small):
+        for k in (1, 3, 40):
+            assert torch.equal(m.generate(idx, 25, top_k=1, draft_model=draft, draft_tokens=k), want)
+    full = m.config.sequence_len - prompt + 1
+    assert torch.equal(m.generate(idx, full, top_k=1, draft_model=m), _greedy(m, idx, full))
+
+
+def test_drafted_sampling_runs_on_its_own_draws():
+    torch.manual_seed(7)
+    m, small = _gpt(), _gpt(layers=1)
+    idx = torch.randint(0, 97, (5, 4))
+    out = m.generate(idx, 30, temperature=0.8, top_k=20, draft_model=small)
+    assert out.shape == (5, 34) and torch.equal(out[:, :4], idx) and 0 <= int(out.min()) and int(out.max()) < 97
+    with pytest.raises(ValueError, match="vocabulary"):
+        m.generate(idx, 3, draft_model=_gpt(vocab=98))
+    with pytest.raises(ValueError):
+        m.generate(idx, 3, draft_model=small, draft_tokens=0)
+    with pytest.raises(ValueError, match="do not fit"):
+        m.generate(idx, 30, draft_model=_gpt(seq=32))
+
+
+@pytest.mark.gpu
+def test_generation_on_the_kernels():
+    """Cached and drafted sampling through all operators.  With a draft that is the model itself nearly everything is accepted: fewer
+    passes, hence fewer kernels, than tokens one by one."""
+    torch.manual_seed(8)
+    m = _gpt(width=256, heads=2, seq=256, vocab=512, device="cuda")
+    idx = torch.randint(0, 512, (4, 30), device="cuda")
+    out = m.generate(idx, 40, top_k=50, use_cache=True)
+    assert out.shape == (4, 70) and torch.equal(out[:, :30], idx)
+    seen = []
+
+    class Counting(GPT):
+        def forward(self, tokens, *a, **kw):
+            seen.append(tokens.numel())
+            return super().forward(tokens, *a, **kw)
+
+    c = Counting(m.config).cuda()
+    c.load_state_dict(m.state_dict())
+    out = c.generate(idx, 40, top_k=50, draft_model=m, draft_tokens=4)
+    ops.check_status()
+    assert out.shape == (4, 70) and 0 <= int(out.min()) and int(out.max()) < 512
+    assert 9 <= len(seen) <= 25  # the prompt, and at least a fifth of 40 tokens
+    big = _llama(width=256, heads=4, kv_heads=2, seq=256, vocab=512, device="cuda")
+    out = big.generate(idx, 20, temperature=0.7, draft_model=_llama(layers=1, width=128, heads=2, kv_heads=1, seq=256, vocab=512, device="cuda"))
+    ops.check_status()
+    assert out.shape == (4, 50)
