@@ -1403,9 +1403,12 @@ Tensor paged_attention(const Tensor& q_, const Tensor& k_pages, const Tensor& v_
   p.q_token = q.stride(0), p.q_head = q.stride(1);
   p.max_new = (int)std::min(max_new, N);
   p.scale = (float)scale;
-  Tensor work = at::empty({dion::paged_attention_workspace(p, (int)D)}, q.options().dtype(at::kByte));
-  DION_CUDA_CHECK(dion::paged_attention_launch(p, (int)D, work.data_ptr(), at::cuda::getCurrentCUDAStream()));
-  g_launches.fetch_add(1, std::memory_order_relaxed);  // the parts are joined by a second one
+  const int64_t bytes = dion::paged_attention_workspace(p, (int)D);
+  Tensor work;
+  if (bytes > 0) work = at::empty({bytes}, q.options().dtype(at::kByte));
+  int launches = 1;
+  DION_CUDA_CHECK(dion::paged_attention_launch(p, (int)D, bytes > 0 ? work.data_ptr() : nullptr, &launches, at::cuda::getCurrentCUDAStream()));
+  g_launches.fetch_add(launches - 1, std::memory_order_relaxed);
   return out;
 }
 

@@ -328,8 +328,8 @@ struct PagedAttention {
 };
 // bytes of `work`, on 16 bytes; needs nothing of what a call before left there
 long long paged_attention_workspace(const PagedAttention& p, int head_dim);
-// two kernels
-cudaError_t paged_attention_launch(const PagedAttention& p, int head_dim, void* work, cudaStream_t stream);
+// launches: set to the number of kernels
+cudaError_t paged_attention_launch(const PagedAttention& p, int head_dim, void* work, int* launches, cudaStream_t stream);
 
 // Drafted tokens against the target's probabilities (verify.cu); rows of `vocab` contiguous floats
 struct VerifyDrafts {

@@ -35,6 +35,7 @@ constexpr int kShareCost = 64;
 struct Tiling {
   int height, tiles, group, subs, heads, tokens;  // heads: kv heads x subs; tokens: of all `tiles`
   int fixed;                                      // what such rows cost apart from their keys, in keys
+  int side = 1;                                   // heads that CTAs next to one another have, see Walk
   FastDiv by_group;
   Tiling() = default;
   Tiling(const PagedAttention& p, int height_, int tiles_, int fixed_) : height(height_), tiles(tiles_), fixed(fixed_) {
@@ -75,6 +76,10 @@ struct Costs {
   __device__ __forceinline__ long long head() const { return items > 0 ? before(items - 1) + fixed + s.cached + s.n : 0; }
 };
 
+// `side` CTAs next to one another have the same share of as many heads next to one another: in a page the rows of these lie side by
+// side, and memory reads them at the same time.  100 sequences of 900 keys, 12 heads of 64, 59 us, a head after the other 71; 48
+// prompts of up to 1024 tokens 98 and 108.
+//
 // Goes through a CTA's share: item `item` of head `head` (of tiling.heads) of sequence b, units begin .. end of its `units` units
 // of K keys.  A share ends inside an item at a whole unit, or, where the item is small against the shares, at its nearer end.
 // Every warp has one in shared memory, which its first lane moves on: in registers it would cost the softmax loops theirs.
@@ -104,8 +109,8 @@ struct Walk {
       if (at >= to) return;
       if ((++item) * (long long)tl.tokens >= n) {
         item = 0;
-        if (++head == tl.heads) {
-          head = 0;
+        if ((head += tl.side) >= tl.heads) {
+          head -= tl.heads;
           Sequence s;
           do {
             if (++b >= p.seqs) {
@@ -141,7 +146,7 @@ __device__ __forceinline__ void my_share(const PagedAttention& p, const Tiling& 
   const int per = (p.seqs + THREADS - 1) / THREADS, t = threadIdx.x, lane = t & 31, warp = t >> 5;
   const int lo = (int)min((long long)t * per, (long long)p.seqs), hi = min(lo + per, p.seqs);
   long long mine = 0;
-  for (int b = lo; b < hi; ++b) mine += Costs(sequence(p, b), tl).head() * tl.heads;
+  for (int b = lo; b < hi; ++b) mine += Costs(sequence(p, b), tl).head() * (tl.heads / tl.side);
   long long upto = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -157,17 +162,18 @@ __device__ __forceinline__ void my_share(const PagedAttention& p, const Tiling& 
     if (i < warp) upto += scratch.sums[i];
     total += scratch.sums[i];
   }
-  const long long ctas = max(1ll, min((long long)gridDim.x, total / kShareCost));
-  const long long each = total / ctas, rest = total - each * ctas;
+  const int shares_most = gridDim.x / tl.side, nth = blockIdx.x / tl.side;
+  const long long shares = max(1ll, min((long long)shares_most, total / kShareCost));
+  const long long each = total / shares, rest = total - each * shares;
   long long from = 0, to = 0;
-  if (blockIdx.x < ctas) {  // total * c / ctas without a product of 64 x 64 bits
-    from = each * blockIdx.x + rest * blockIdx.x / ctas;
-    to = each * (blockIdx.x + 1) + rest * (blockIdx.x + 1) / ctas;
+  if (nth < shares) {  // total * nth / shares without a product of 64 x 64 bits
+    from = each * nth + rest * nth / shares;
+    to = each * (nth + 1) + rest * (nth + 1) / shares;
   }
   if (from < to && upto - mine <= from && from < upto) {  // the thread whose sequences hold the start
     long long at = upto - mine;
     for (int b = lo; b < hi; ++b) {
-      const long long cost = Costs(sequence(p, b), tl).head() * tl.heads;
+      const long long cost = Costs(sequence(p, b), tl).head() * (tl.heads / tl.side);
       if (from < at + cost) {
         scratch.b = b;
         scratch.start = at;
@@ -187,8 +193,9 @@ __device__ __forceinline__ void my_share(const PagedAttention& p, const Tiling& 
       const Sequence s = sequence(p, w.b);
       w.take(s);
       const Costs c(s, tl);
-      w.head = (int)((from - w.at) / c.head());
-      w.at += w.head * c.head();
+      const int before = (int)((from - w.at) / c.head());
+      w.head = before * tl.side + blockIdx.x % tl.side;
+      w.at += before * c.head();
       int low = 0, high = c.items;  // the item that holds the start
       while (high - low > 1) {
         const int mid = (low + high) / 2;
@@ -209,13 +216,14 @@ __device__ __forceinline__ void my_share(const PagedAttention& p, const Tiling& 
 // later CTA ends it.
 struct Share {
   int b, head, item;  // in slot 2c + 1; b = -1: none
-  short continues;    // slot 2c is filled; -1: the share has not one unit
+  short continues;    // slot 2c is filled; -1: the share has not one unit, and the slot says that it has no part in anything
   short ends;         // slot 2c's item ends here
 };
 struct Parts {
   float* acc;    // [slot][rows of an item][head_dim], not normalised
   float2* ml;    // [slot][rows of an item]: maximum (log2 units) and sum
   Share* share;  // per CTA
+  int cluster, items;  // where a cluster has an item: its CTAs, and items of a sequence and head
 };
 
 // Row r of an item: its token in the sequence and its query head; false where there is none
@@ -234,13 +242,16 @@ constexpr int kKeys = 64;               // keys of a stage
 // What an item costs apart from its keys, in keys: the first load's way, the warps' join, the result.  200 sequences of up to 200
 // keys, 32 heads on 8 (us): 79 at 0, 34 at 128, 28 at 256, 30 at 512; where all are long it makes no difference.
 constexpr int kRowsFixed = 256;
+constexpr int kFewCluster = 8;        // CTAs of a cluster that has one item, at most
+constexpr int kFewItems = 1 << 20;   // items of such a launch, at most
 constexpr int kRowsThreads = 32 * 5;    // four warps of products and one that loads
 
-template <int D_, int WM_>
+template <int D_, int WM_, bool FEW_>
 struct Rows {
   static constexpr int D = D_, WM = WM_, WK = 4 / WM, TR = 16 * WM;  // warps along the rows and along the keys, rows of a tile
+  static constexpr bool FEW = FEW_;  // an item per cluster
   static constexpr int PANELS = D / 64, PANEL = kKeys * 128, STAGE = 2 * PANELS * PANEL;  // bytes; K panels, then V panels
-  static constexpr int STAGES = D == 128 ? 3 : 6;
+  static constexpr int STAGES = D == 128 ? 3 : FEW ? 4 : 6;
   static constexpr int EXCHANGE = WK > 1 ? 2 * 16 * D * 4 : 0;  // accumulators of two warps on their way to their neighbours
   static constexpr int SMEM = STAGES * STAGE + EXCHANGE + 1024;
   static_assert(SMEM <= 115712, "two CTAs per SM");
@@ -276,10 +287,47 @@ __device__ __forceinline__ float quad_sum(float v) {
 }
 __device__ __forceinline__ void products_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }  // the four warps of products
 
+__device__ __forceinline__ float4 remote4(const float* v, int rank) {
+  float4 r;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(r.x), "=f"(r.y), "=f"(r.z), "=f"(r.w)
+               : "r"(mapa_shared(smem_u32(v), (uint32_t)rank))
+               : "memory");
+  return r;
+}
+__device__ __forceinline__ float2 remote2(const void* v, int rank) {
+  float2 r;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(r.x), "=f"(r.y) : "r"(mapa_shared(smem_u32(v), (uint32_t)rank)) : "memory");
+  return r;
+}
+
+// Writes zeros to rows that are nobody's (behind the last sequence, of wrong ones) and reports what is wrong with the sequences: the
+// part of block `block` of `blocks`, by threads `t` of `threads`.
+template <int D>
+__device__ __forceinline__ void nobodys_rows(const PagedAttention& p, int block, int blocks, int t, int threads) {
+  auto clear = [&](long long lo, long long hi) {
+    lo = max(lo, 0ll);
+    hi = min(hi, (long long)p.tokens);
+    const long long per_row = (long long)p.heads * D / 8;
+    for (long long i = lo * per_row + t; i < hi * per_row; i += threads) reinterpret_cast<uint4*>(p.out)[i] = make_uint4(0, 0, 0, 0);
+  };
+  for (int b = block; b < p.seqs; b += blocks) {
+    if (sequence(p, b).bad) {
+      if (t == 0) bad_argument(p.status);
+      clear(p.offsets[b], p.offsets[b + 1]);
+    }
+  }
+  if (block == 0 && t == 0 && p.offsets[0] != 0) bad_argument(p.status);
+  for (long long r = max(0ll, (long long)p.offsets[p.seqs]) + block; r < p.tokens; r += blocks) clear(r, r + 1);
+}
+
 // Bound by the bandwidth of the cache: 64 keys are 32 KB (head dimension 128), which an SM gets in 1400 cycles, and take four
 // warps some 600.  So the legacy products, whose tiles are 16 rows high, do: the rows of single tokens fill no more.  A warp loads
 // 64 keys a stage by TMA, the boxes of several pages where they are smaller; where the rows fit one 16-row tile the four others
 // take 16 keys each and join their sums per item, else they share the keys and have rows of their own.
+//
+// FEW: a cluster has one item, its CTAs equal parts of the keys, and the parts are joined over the cluster's shared memory.  That
+// saves the second kernel where items are short; what counts there is the chain of latencies.
 template <typename C>
 __global__ void __launch_bounds__(kRowsThreads, 2)
 paged_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const PagedAttention p,
@@ -298,7 +346,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
   if (smem_u32(smem) & 1023) {  // the 128-byte swizzle repeats every 1024 bytes
     if (threadIdx.x == 0) {
       bad_argument(p.status);
-      parts.share[blockIdx.x] = Share{-1, 0, 0, -1, 0};
+      if (!C::FEW) parts.share[blockIdx.x] = Share{-1, 0, 0, -1, 0};
     }
     return;
   }
@@ -315,7 +363,30 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
   pdl_trigger();
   pdl_wait();
   Walk<kKeys>& w = walks[warp];
-  my_share(p, tl, *scratch, w);
+  const int rank = C::FEW ? (int)blockIdx.x % parts.cluster : 0;
+  if constexpr (C::FEW) {
+    if (lane == 0) {
+      Walk<kKeys> mine{};
+      const int nth = (int)blockIdx.x / parts.cluster, seq_item = nth / tl.heads;
+      mine.head = nth - seq_item * tl.heads;
+      mine.b = seq_item / parts.items;
+      mine.item = seq_item - mine.b * parts.items;
+      const Sequence s = sequence(p, mine.b);
+      mine.take(s);
+      const Costs c(s, tl);
+      if (mine.item < c.items) {
+        mine.to = 1;  // valid
+        mine.keys = c.keys(mine.item);
+        mine.units = (mine.keys + kKeys - 1) / kKeys;
+        mine.begin = (int)((long long)mine.units * rank / parts.cluster);
+        mine.end = (int)((long long)mine.units * (rank + 1) / parts.cluster);
+      }
+      w = mine;
+    }
+    __syncthreads();
+  } else {
+    my_share(p, tl, *scratch, w);
+  }
   Ring<C::STAGES> ring;
 
   if (warp == 4) {
@@ -358,8 +429,9 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
         }
         ring.next();
       }
-      if (__any_sync(0xffffffffu, *abort_flag != 0)) break;
+      if (C::FEW || __any_sync(0xffffffffu, *abort_flag != 0)) break;
     }
+    if (C::FEW) nobodys_rows<D>(p, blockIdx.x, gridDim.x, lane, 32);
   } else {
     // ------------------------------------------------------------------ products
     // A wait that gives up raises the abort flag and the warp goes on without waiting, so that the barriers of the four are met.
@@ -517,6 +589,20 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
         }
       }
       const bool starts = w.begin == 0, ends = w.end == w.units;
+      if (C::FEW && parts.cluster > 1) {
+        products_sync();  // nobody reads the ring or the statistics any more: the sums go there
+        if (wk == 0) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int r = wm * 16 + quad + 8 * i;
+            if ((lane & 3) == 0) stats[r] = make_float2(m[i], l[i]);
+#pragma unroll
+            for (int c = 0; c < D / 8; ++c)
+              *reinterpret_cast<float2*>(reinterpret_cast<float*>(smem) + r * D + c * 8 + pair) = make_float2(o[c][2 * i], o[c][2 * i + 1]);
+          }
+        }
+        break;
+      }
       if (wk == 0) {
         if (starts && ends) {
 #pragma unroll
@@ -543,8 +629,46 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
       if (starts && !ends) share.b = w.b, share.head = w.head, share.item = w.item;
       if (first_item) share.continues = !starts, share.ends = ends;
       first_item = false;
+      if (C::FEW) break;
     }
-    if (threadIdx.x == 0) parts.share[blockIdx.x] = share;
+    if (!C::FEW) {
+      if (threadIdx.x == 0) parts.share[blockIdx.x] = share;
+      if (share.continues < 0 && threadIdx.x < TR) parts.ml[2ll * blockIdx.x * TR + threadIdx.x] = make_float2(-INFINITY, 0.f);
+    }
+  }
+  if (C::FEW && parts.cluster > 1 && w.valid()) {  // the same in all CTAs of the cluster
+    cluster_sync_all();
+    for (int r = rank + parts.cluster * warp; r < tl.height; r += parts.cluster * (kRowsThreads / 32)) {
+      int token, h;
+      if (!row_of(p, tl, w.n, w.head, w.item, 0, r, token, h)) continue;
+      const float2 t = lane < parts.cluster ? remote2(&stats[r], lane) : make_float2(-INFINITY, 0.f);
+      float top = t.x;
+#pragma unroll
+      for (int o = 4; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      top = __shfl_sync(0xffffffffu, top, 0);  // of the first eight lanes; the row sees a key, so some part has one
+      const float f = fast_exp2(t.x - top);
+      float sum = t.y * f;
+#pragma unroll
+      for (int o = 4; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      const float inv = 1.f / __shfl_sync(0xffffffffu, sum, 0);
+      const float* acc = reinterpret_cast<const float*>(smem) + r * D + lane * (D / 32);
+      float v[D / 32] = {};
+#pragma unroll 8
+      for (int k = 0; k < parts.cluster; ++k) {
+        const float fk = __shfl_sync(0xffffffffu, f, k);
+        if constexpr (D == 128) {
+          const float4 a = remote4(acc, k);
+          v[0] += a.x * fk, v[1] += a.y * fk, v[2] += a.z * fk, v[3] += a.w * fk;
+        } else {
+          const float2 a = remote2(acc, k);
+          v[0] += a.x * fk, v[1] += a.y * fk;
+        }
+      }
+      bf16* dst = p.out + ((long long)(w.first + token) * p.heads + h) * D + lane * (D / 32);
+#pragma unroll
+      for (int i = 0; i < D / 32; i += 2) *reinterpret_cast<uint32_t*>(dst + i) = pack_bf16x2(v[i] * inv, v[i + 1] * inv);
+    }
+    cluster_sync_all();  // nobody reads another's shared memory after this
   }
   __syncthreads();
   if (*abort_flag != 0) {
@@ -554,109 +678,107 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
   }
 }
 
-// Joins the parts of items that several CTAs had, writes zeros to rows that are nobody's and reports what is wrong with the
-// sequences.  Block (c, y) has the item that CTA c began, and of its rows as many at a time as it has groups of WPR warps; the
-// warps of a group share the parts.  Few rows come in many parts (a cache of 4000 keys over the whole GPU in 30), so eight warps
-// take a row together there; many rows come in two or three, and a warp takes each.
-template <int D, int WPR>
-__global__ void __launch_bounds__(256) paged_join_kernel(const PagedAttention p, const Parts parts, const __grid_constant__ Tiling tl) {
-  constexpr int E = D / 32, ROWS = 8 / WPR;  // columns of a lane, rows of a block at a time
-  __shared__ float sums[WPR > 1 ? WPR : 1][D + 2];
+// Joins the parts of items that several CTAs had and sees to nobody's rows.  Block (c, y) has the item that CTA c began, and of its
+// rows as many at a time as it has groups of WPR warps; the warps of a group share the parts.  Few rows come in many parts (a cache of
+// 4000 keys over the whole GPU in 30), so four warps take a row together there; many rows come in two or three, and a warp takes
+// each.  Bound by latency: what the next step needs is loaded before this one has decided whether, and the code is kept short, as
+// every call fetches it anew.
+template <int D, int WPR, int ROWS>
+__global__ void __launch_bounds__(32 * WPR * ROWS) paged_join_kernel(const PagedAttention p, const Parts parts, const __grid_constant__ Tiling tl) {
+  constexpr int E = D / 32, AT_ONCE = WPR > 1 ? 4 : 2;  // columns of a lane, parts whose loads are under way at once
+  __shared__ float sums[WPR][D + 2];
   pdl_trigger();
   pdl_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = blockIdx.x, ctas = gridDim.x, rows = tl.height * tl.tiles;
+  const int side = tl.side;  // CTAs c, c + side ... have the item's parts
   const Share mine = parts.share[c];
-  if (blockIdx.y == 0) {  // sequences c, c + ctas ... and a share of the rows behind the last
-    auto clear = [&](long long lo, long long hi) {
-      lo = max(lo, 0ll);
-      hi = min(hi, (long long)p.tokens);
-      const long long per_row = (long long)p.heads * D / 8;
-      for (long long i = lo * per_row + threadIdx.x; i < hi * per_row; i += 256) reinterpret_cast<uint4*>(p.out)[i] = make_uint4(0, 0, 0, 0);
-    };
-    for (int b = c; b < p.seqs; b += ctas) {
-      if (sequence(p, b).bad) {
-        if (threadIdx.x == 0) bad_argument(p.status);
-        clear(p.offsets[b], p.offsets[b + 1]);
-      }
-    }
-    if (c == 0 && threadIdx.x == 0 && p.offsets[0] != 0) bad_argument(p.status);
-    for (long long r = max(0ll, (long long)p.offsets[p.seqs]) + c; r < p.tokens; r += ctas) clear(r, r + 1);
-  }
-  if (mine.b < 0) return;
-  const Sequence s = sequence(p, mine.b);
-  int last = c;  // the CTA that ends the item
+  int last = 0;  // how many of them until the one that ends it
   for (bool more = true; more;) {
-    const int i = last + 1 + lane;
-    const bool stop = i >= ctas || parts.share[i].continues == 0 || (parts.share[i].continues > 0 && parts.share[i].ends);
-    const unsigned at = __ballot_sync(0xffffffffu, stop);
-    more = at == 0;
+    const int i = c + (last + 1 + lane) * side;
+    const Share s = parts.share[min(i, ctas - 1)];
+    const unsigned at = __ballot_sync(0xffffffffu, i >= ctas || s.continues == 0 || (s.continues > 0 && s.ends));
+    more = at == 0 && mine.b >= 0;
     last += more ? 32 : __ffs(at);
   }
-  last = min(last, ctas - 1);
-  const int sub = warp % WPR;
-  for (int r = blockIdx.y * ROWS + warp / WPR; r < rows; r += ROWS * gridDim.y) {
-    int token, h;
-    if (!row_of(p, tl, s.n, mine.head, mine.item, r / tl.height, r % tl.height, token, h)) continue;  // all warps of the row
-    float top = -INFINITY, sum = 0.f, acc[E];
+  last = min(last, (ctas - 1 - c) / side);
+  if (mine.b >= 0) {
+    const Sequence s = sequence(p, mine.b);
+    const int sub = warp % WPR;
+    for (int r = blockIdx.y * ROWS + warp / WPR; r < rows; r += ROWS * gridDim.y) {
+      int token, h;
+      if (!row_of(p, tl, s.n, mine.head, mine.item, r / tl.height, r % tl.height, token, h)) continue;  // all warps of the row
+      float top = -INFINITY, sum = 0.f, acc[E];
 #pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = 0.f;
-    // this warp's parts are those of CTAs c + sub, c + sub + WPR ..., 32 at a time
-    for (int base = c + sub; base <= last; base += 32 * WPR) {
-      const int i = base + lane * WPR;
-      const long long slot = i == c ? 2ll * c + 1 : 2ll * i;
-      const bool has = i == c || (i <= last && parts.share[i].continues > 0);
-      const float2 t = has ? parts.ml[slot * rows + r] : make_float2(-INFINITY, 0.f);
-      float most = t.x;
+      for (int e = 0; e < E; ++e) acc[e] = 0.f;
+      auto slot = [&](int nth) { return (2 * (c + (long long)nth * side) + (nth == 0 ? 1 : 0)) * rows + r; };
+      // this warp's parts are numbers sub, sub + WPR ..., 32 at a time
+      for (int base = sub; base <= last; base += 32 * WPR) {
+        const int nth = base + lane * WPR, n = min(32, (last - base) / WPR + 1);
+        const float2 t = nth <= last ? parts.ml[slot(nth)] : make_float2(-INFINITY, 0.f);
+        float most = t.x;
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-      const float top2 = fmaxf(top, most), neg = top2 == -INFINITY ? 0.f : -top2, f = fast_exp2(top + neg), mw = fast_exp2(t.x + neg);
-      float part = t.y * mw;
+        for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+        const float top2 = fmaxf(top, most), neg = top2 == -INFINITY ? 0.f : -top2, f = fast_exp2(top + neg), w = fast_exp2(t.x + neg);
+        sum = sum * f + t.y * w;  // of this lane's parts
+        top = top2;
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
-      sum = sum * f + part;
-      top = top2;
+        for (int e = 0; e < E; ++e) acc[e] *= f;
+#pragma unroll 1
+        for (int k = 0; k < n; k += AT_ONCE) {
+          float v[AT_ONCE][E];
 #pragma unroll
-      for (int e = 0; e < E; ++e) acc[e] *= f;
-      const int n = min(32, (last - base) / WPR + 1);
-#pragma unroll 4
-      for (int k = 0; k < n; ++k) {
-        const float wk = __shfl_sync(0xffffffffu, mw, k);
-        const int j = base + k * WPR;
-        const long long from = (j == c ? 2ll * c + 1 : 2ll * j) * rows + r;
-        if (wk > 0.f) {  // a part that saw none of the row's keys, or a share without units, has nothing written
+          for (int j = 0; j < AT_ONCE; ++j) {
+            const float* from = parts.acc + slot(base + min(k + j, n - 1) * WPR) * D + lane * E;
+            if constexpr (E == 4) {
+              const float4 x = *reinterpret_cast<const float4*>(from);
+              v[j][0] = x.x, v[j][1] = x.y, v[j][2] = x.z, v[j][3] = x.w;
+            } else {
+              const float2 x = *reinterpret_cast<const float2*>(from);
+              v[j][0] = x.x, v[j][1] = x.y;
+            }
+          }
 #pragma unroll
-          for (int e = 0; e < E; ++e) acc[e] += wk * parts.acc[from * D + e * 32 + lane];
+          for (int j = 0; j < AT_ONCE; ++j) {
+            const float wj = __shfl_sync(0xffffffffu, w, (k + j) & 31);
+            if (k + j < n && wj > 0.f) {  // a part that saw none of the row's keys has nothing written
+#pragma unroll
+              for (int e = 0; e < E; ++e) acc[e] += wj * v[j][e];
+            }
+          }
         }
       }
-    }
-    if constexpr (WPR > 1) {
-      if (lane == 0) sums[sub][D] = top, sums[sub][D + 1] = sum;
 #pragma unroll
-      for (int e = 0; e < E; ++e) sums[sub][e * 32 + lane] = acc[e];
-      __syncthreads();
-      if (sub == 0) {
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if constexpr (WPR > 1) {
+        if (lane == 0) sums[sub][D] = top, sums[sub][D + 1] = sum;
 #pragma unroll
-        for (int i = 1; i < WPR; ++i) top = fmaxf(top, sums[i][D]);
-        sum = 0.f;
+        for (int e = 0; e < E; ++e) sums[sub][lane * E + e] = acc[e];
+        __syncthreads();
+        const float mine_top = top;
+#pragma unroll 1
+        for (int i = 0; i < WPR; ++i) top = fmaxf(top, sums[i][D]);
+        float f = fast_exp2(mine_top - top);
+        sum *= f;
 #pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] = 0.f;
-#pragma unroll
-        for (int i = 0; i < WPR; ++i) {
-          const float f = fast_exp2(sums[i][D] - (top == -INFINITY ? 0.f : top));
+        for (int e = 0; e < E; ++e) acc[e] *= f;
+#pragma unroll 1
+        for (int i = 1; i < WPR; ++i) {  // only the first warp's result counts
+          f = fast_exp2(sums[i][D] - top);
           sum += sums[i][D + 1] * f;
 #pragma unroll
-          for (int e = 0; e < E; ++e) acc[e] += sums[i][e * 32 + lane] * f;
+          for (int e = 0; e < E; ++e) acc[e] += sums[i][lane * E + e] * f;
         }
       }
-    }
-    if (sub == 0) {
-      const float inv = sum > 0.f ? 1.f / sum : 0.f;
+      if (sub == 0) {
+        const float inv = sum > 0.f ? 1.f / sum : 0.f;
+        bf16* dst = p.out + ((long long)(s.first + token) * p.heads + h) * D + lane * E;
 #pragma unroll
-      for (int e = 0; e < E; ++e)
-        p.out[((long long)(s.first + token) * p.heads + h) * D + e * 32 + lane] = __float2bfloat16(acc[e] * inv);
+        for (int e = 0; e < E; e += 2) *reinterpret_cast<uint32_t*>(dst + e) = pack_bf16x2(acc[e] * inv, acc[e + 1] * inv);
+      }
+      if constexpr (WPR > 1) __syncthreads();
     }
-    if constexpr (WPR > 1) __syncthreads();
   }
+  if (blockIdx.y == 0) nobodys_rows<D>(p, c, ctas, threadIdx.x, 32 * WPR * ROWS);
 }
 
 // ---------------------------------------------------------------------------------- many rows: tcgen05
@@ -1046,6 +1168,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
       first_item = false;
     }
     if (threadIdx.x == 128) parts.share[blockIdx.x] = share;
+    if (share.continues < 0) parts.ml[2ll * blockIdx.x * (2 * kBM) + x * kBM + row_in_tile] = make_float2(-INFINITY, 0.f);
     if (*abort_flag != 0 && lane == 0) atomicCAS(p.status, 0, kStatusEpilogueTimeout);
   }
 
@@ -1106,12 +1229,32 @@ bool queries_tmap(CUtensorMap* map, const PagedAttention& p, int head_dim, const
 // caller knows less.
 struct Plan {
   Tiling tl;
-  int ctas;
-  explicit Plan(const PagedAttention& p) {
+  int ctas, cluster = 0, items = 0;  // cluster > 0: CTAs of an item, and the items that a sequence and head can have
+  Plan(const PagedAttention& p, int head_dim) {
     const long long group = p.heads / p.kv_heads, typical = (2ll * p.tokens + p.seqs - 1) / p.seqs;
     const long long rows = std::min<long long>(p.max_new, typical) * group;
+    const int sms = attn_grid(1 << 20);
     tl = rows <= 64 ? Tiling(p, rows <= 16 ? 16 : rows <= 32 ? 32 : 64, 1, kRowsFixed) : Tiling(p, kBM, 2, kChunkFixed);
-    ctas = attn_grid(1 << 20) * (tl.tiles == 1 ? 2 : 1);
+    ctas = sms * (tl.tiles == 1 ? 2 : 1);
+    for (int h = 1; h <= tl.heads && h <= ctas; ++h)
+      if (tl.heads % h == 0 && ctas % h == 0) tl.side = h;
+    if (tl.tiles > 1) return;
+    // An item per cluster, without a second kernel, where the keys of its CTAs are few even if a sequence fills its row of the
+    // page table, which is all that the host knows: at most 4096 each, or 1024 where the clusters leave half of the SMs idle.  Both ways
+    // (us, shares / clusters; 32 heads on 8 of 128): one token over 1000 keys 12.0 / 6.9, over 4000 13.7 / 9.0, over 16000 17.5 / 20.5;
+    // 8 of 8000 52.0 / 44.7, 32 of up to 4000 54.2 / 48.2, 64 of 1000 54.7 / 46.0, 64 of 4000 165.7 / 149.5; of 8000 keys a CTA 40 items
+    // 201 / 227, 64 of up to 8000 138 / 131.
+    const long long most = (p.max_new + tl.tokens - 1) / tl.tokens, all = (long long)p.seqs * tl.heads * most;
+    const long long keys = (long long)p.max_pages << p.page_shift, slots = (long long)sms * (head_dim == 64 ? 3 : 2);
+    for (int c = kFewCluster; c >= 1; c /= 2) {
+      if (c > 1 ? all * c > slots : all > kFewItems) continue;
+      if (keys <= c * (2 * all * c < slots ? 1024ll : 4096ll)) {
+        cluster = c;
+        items = (int)most;
+        ctas = (int)all * c;
+      }
+      break;
+    }
   }
   int rows() const { return tl.height * tl.tiles; }
 };
@@ -1127,7 +1270,14 @@ cudaError_t rows_launch(const PagedAttention& p, const Parts& parts, const Plan&
     return cudaFuncSetAttribute(paged_rows_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
   });
   if (e != cudaSuccess) return e;
-  return launch_pdl(paged_rows_kernel<C>, dim3(plan.ctas), dim3(kRowsThreads), C::SMEM, stream, 0, tk, tv, p, parts, plan.tl);
+  return launch_pdl(paged_rows_kernel<C>, dim3(plan.ctas), dim3(kRowsThreads), C::SMEM, stream, C::FEW && plan.cluster > 1 ? plan.cluster : 0, tk, tv,
+                    p, parts, plan.tl);
+}
+template <int D, bool FEW>
+cudaError_t rows_launch_d(const PagedAttention& p, const Parts& parts, const Plan& plan, cudaStream_t stream) {
+  return plan.rows() == 16   ? rows_launch<Rows<D, 1, FEW>>(p, parts, plan, stream)
+         : plan.rows() == 32 ? rows_launch<Rows<D, 2, FEW>>(p, parts, plan, stream)
+                             : rows_launch<Rows<D, 4, FEW>>(p, parts, plan, stream);
 }
 
 template <int D>
@@ -1151,34 +1301,38 @@ cudaError_t chunk_launch(const PagedAttention& p, const Parts& parts, const Plan
 }
 
 template <int D>
-cudaError_t attention_launch(const PagedAttention& p, void* work, cudaStream_t stream) {
-  const Plan plan(p);
-  Parts parts;
+cudaError_t attention_launch(const PagedAttention& p, void* work, int* launches, cudaStream_t stream) {
+  const Plan plan(p, D);
+  *launches = plan.cluster > 0 ? 1 : 2;
+  Parts parts{};
+  if (plan.cluster > 0) {
+    parts.cluster = plan.cluster;
+    parts.items = plan.items;
+    return rows_launch_d<D, true>(p, parts, plan, stream);
+  }
   parts.acc = reinterpret_cast<float*>(work);
   parts.ml = reinterpret_cast<float2*>(parts.acc + 2ll * plan.ctas * plan.rows() * D);
   parts.share = reinterpret_cast<Share*>(parts.ml + 2ll * plan.ctas * plan.rows());
-  const cudaError_t e = plan.rows() == 16   ? rows_launch<Rows<D, 1>>(p, parts, plan, stream)
-                        : plan.rows() == 32 ? rows_launch<Rows<D, 2>>(p, parts, plan, stream)
-                        : plan.rows() == 64 ? rows_launch<Rows<D, 4>>(p, parts, plan, stream)
-                                            : chunk_launch<D>(p, parts, plan, stream);
+  const cudaError_t e = plan.tl.tiles == 1 ? rows_launch_d<D, false>(p, parts, plan, stream) : chunk_launch<D>(p, parts, plan, stream);
   if (e != cudaSuccess) return e;
   // of a tile's rows those that a sequence can have
   const long long most = std::min<long long>(plan.rows(), (long long)p.max_new * (p.heads / p.kv_heads));
   if (plan.tl.tiles == 1)
-    return launch_pdl(paged_join_kernel<D, 8>, dim3(plan.ctas, (unsigned)std::min<long long>(most, 16)), dim3(256), 0, stream, 0, p, parts, plan.tl);
-  return launch_pdl(paged_join_kernel<D, 1>, dim3(plan.ctas, 16), dim3(256), 0, stream, 0, p, parts, plan.tl);
+    return launch_pdl(paged_join_kernel<D, 4, 1>, dim3(plan.ctas, (unsigned)std::min<long long>(most, 16)), dim3(128), 0, stream, 0, p, parts, plan.tl);
+  return launch_pdl(paged_join_kernel<D, 1, 8>, dim3(plan.ctas, 16), dim3(256), 0, stream, 0, p, parts, plan.tl);
 }
 
 }  // namespace
 
 long long paged_attention_workspace(const PagedAttention& p, int head_dim) {
-  const Plan plan(p);
+  const Plan plan(p, head_dim);
+  if (plan.cluster > 0) return 0;
   return 2ll * plan.ctas * plan.rows() * (head_dim * sizeof(float) + sizeof(float2)) + plan.ctas * sizeof(Share);
 }
 
-cudaError_t paged_attention_launch(const PagedAttention& p, int head_dim, void* work, cudaStream_t stream) {
-  if (head_dim == 64) return attention_launch<64>(p, work, stream);
-  if (head_dim == 128) return attention_launch<128>(p, work, stream);
+cudaError_t paged_attention_launch(const PagedAttention& p, int head_dim, void* work, int* launches, cudaStream_t stream) {
+  if (head_dim == 64) return attention_launch<64>(p, work, launches, stream);
+  if (head_dim == 128) return attention_launch<128>(p, work, launches, stream);
   return cudaErrorInvalidValue;
 }
 

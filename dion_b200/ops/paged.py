@@ -29,12 +29,16 @@ from . import runtime
 
 
 def _no_gradients(name: str, *tensors: Optional[torch.Tensor]) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError(f"{name} has no gradient: call it under torch.no_grad() or with detached inputs")
+    for t in tensors:
+        if t is not None and t.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError(f"{name} has no gradient: call it under torch.no_grad() or with detached inputs")
 
 
 def _on_kernels(q: torch.Tensor) -> bool:
-    return q.is_cuda and q.dtype == torch.bfloat16 and q.shape[-1] in (64, 128) and runtime.use_cuda_kernels(q)
+    return q.is_cuda and q.dtype is torch.bfloat16 and q.shape[-1] in (64, 128) and runtime.use_cuda_kernels(q)
+
+
+_OPS = torch.ops.dion_b200  # the operators are looked up on it at the first call, when the library has been loaded
 
 
 # --------------------------------------------------------------------------- plain path
@@ -159,8 +163,8 @@ def paged_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.T
     if norm_eps is not None and not norm_eps >= 0.0:
         raise ValueError(f"paged_append: norm_eps is None or not negative, not {norm_eps}")
     if _on_kernels(q):
-        return torch.ops.dion_b200.paged_append(q, k, v, cos, sin, k_pages, v_pages, page_table, new_offsets, lengths,
-                                                -1.0 if norm_eps is None else norm_eps, runtime.status_tensor(q.device))
+        return _OPS.paged_append(q, k, v, cos, sin, k_pages, v_pages, page_table, new_offsets, lengths,
+                                 -1.0 if norm_eps is None else norm_eps, runtime.status_tensor(q.device))
     return _append_plain(q, k, v, cos, sin, k_pages, v_pages, page_table, new_offsets, lengths, norm_eps)
 
 
@@ -182,8 +186,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     elif max_new < 1:
         raise ValueError(f"paged_attention: max_new is at least 1, not {max_new}")
     if _on_kernels(q):
-        return torch.ops.dion_b200.paged_attention(q, k_pages, v_pages, page_table, new_offsets, lengths, scale, max_new,
-                                                   runtime.status_tensor(q.device))
+        return _OPS.paged_attention(q, k_pages, v_pages, page_table, new_offsets, lengths, scale, max_new,
+                                    runtime.status_tensor(q.device))
     return _attention_plain(q, k_pages, v_pages, page_table, new_offsets, lengths, scale, max_new)
 
 
@@ -200,9 +204,7 @@ def verify_drafts(target_probs: torch.Tensor, draft_probs: Optional[torch.Tensor
     numbers count as zero there, and a row of zeros gives token 0.  Returns ``(accepted, token)``, int64 per sequence."""
     _no_gradients("verify_drafts", target_probs, draft_probs, uniforms)
     if target_probs.is_cuda and runtime.use_cuda_kernels(target_probs):
-        accepted, token = torch.ops.dion_b200.verify_drafts(target_probs, draft_probs, draft_tokens, uniforms,
-                                                            runtime.status_tensor(target_probs.device))
-        return accepted, token
+        return _OPS.verify_drafts(target_probs, draft_probs, draft_tokens, uniforms, runtime.status_tensor(target_probs.device))
     p, q = target_probs, draft_probs
 
     def need(ok, what):

@@ -177,8 +177,9 @@ def _check_attention(got, q, c, scale=None):
 @pytest.mark.parametrize("sizes", list(SIZES))
 @pytest.mark.parametrize("heads,kv_heads,dim,page,order", [
     (6, 6, 128, 64, "rows"), (12, 12, 64, 16, "heads"), (32, 8, 128, 16, "heads"), (6, 2, 64, 32, "rows"), (8, 1, 128, 256, "heads"), (5, 1, 64, 16, "rows")])
-def test_attention(device, sizes, heads, kv_heads, dim, page, order):
-    c = Paged(SIZES[sizes], heads, kv_heads, dim, page, device, order=order, tail=2).fill()
+@pytest.mark.parametrize("wide", [3, 5000])  # columns of the page table that no sequence reaches
+def test_attention(device, sizes, heads, kv_heads, dim, page, order, wide):
+    c = Paged(SIZES[sizes], heads, kv_heads, dim, page, device, order=order, tail=2, wide=wide).fill()
     q = torch.randn(c.tokens, heads, dim, device=device).bfloat16() * 1.5
     for most in (None, max(n for _, n in c.sizes) or 1):
         got = ops.paged_attention(q, *c.where(), max_new=most)
@@ -192,9 +193,10 @@ def test_attention(device, sizes, heads, kv_heads, dim, page, order):
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("heads,kv_heads", [(1, 1), (17, 1), (64, 1), (71, 1), (130, 1), (40, 20), (9, 3)])
 @pytest.mark.parametrize("new", [1, 3, 40])
-def test_attention_of_any_group(device, heads, kv_heads, new):
+@pytest.mark.parametrize("wide", [3, 5000])
+def test_attention_of_any_group(device, heads, kv_heads, new, wide):
     """Groups of heads that fill no tile, and ones larger than one."""
-    c = Paged([(100, new), (0, new), (37, 1)], heads, kv_heads, 64, 16, device, order="heads").fill()
+    c = Paged([(100, new), (0, new), (37, 1)], heads, kv_heads, 64, 16, device, order="heads", wide=wide).fill()
     q = torch.randn(c.tokens, heads, 64, device=device).bfloat16()
     got = ops.paged_attention(q, *c.where(), max_new=new)
     if device == "cuda":
@@ -211,8 +213,9 @@ def test_attention_of_any_group(device, heads, kv_heads, new):
     ([(i * 7 % 900, 1 + (i % 5 == 0) * 2) for i in range(200)], 12, 4, 64, 16),
     ([(0, 1)] * 1500, 2, 2, 64, 16),                          # more sequences than threads of a block
 ])
-def test_attention_split_over_the_gpu(sizes, heads, kv_heads, dim, page):
-    c = Paged(sizes, heads, kv_heads, dim, page, "cuda", order="heads").fill()
+@pytest.mark.parametrize("wide", [0, 5000])
+def test_attention_split_over_the_gpu(sizes, heads, kv_heads, dim, page, wide):
+    c = Paged(sizes, heads, kv_heads, dim, page, "cuda", order="heads", wide=wide).fill()
     q = torch.randn(c.tokens, heads, dim, device="cuda").bfloat16()
     first = ops.paged_attention(q, *c.where())
     _check_attention(first, q, c)
@@ -222,10 +225,11 @@ def test_attention_split_over_the_gpu(sizes, heads, kv_heads, dim, page):
 
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("new", [1, 90])
-def test_attention_of_large_and_small_scores(device, new):
+@pytest.mark.parametrize("wide", [3, 5000])
+def test_attention_of_large_and_small_scores(device, new, wide):
     """Scores that grow along the sequence, so that the running maximum moves at every step, far from zero on either side, and all
     equal: the weights are exact multiples then."""
-    c = Paged([(700, new)], 4, 2, 64, 16, device).fill()
+    c = Paged([(700, new)], 4, 2, 64, 16, device, wide=wide).fill()
     page, row = c.slots(0, 0, 700 + new)
     ramp = torch.linspace(-6, 6, 700 + new, device=device)[:, None, None].expand(-1, 2, 64)
     q = torch.ones(new, 4, 64, device=device).bfloat16() * 5
@@ -442,7 +446,7 @@ def _bad(device):
 
     return [("a page below", lambda c: table(c, 1, 1, -1)), ("a page beyond", lambda c: table(c, 0, 1, c.k.shape[0])),
             ("a page far beyond", lambda c: table(c, 1, 1, 2 ** 31 - 1)),
-            ("a length below zero", lambda c: dict(lengths=ints(20, -1))), ("a length beyond the table", lambda c: dict(lengths=ints(20, 16 * 40))),
+            ("a length below zero", lambda c: dict(lengths=ints(20, -1))), ("a length beyond the table", lambda c: dict(lengths=ints(20, 16 * c.table.shape[1] - 1))),
             ("the largest length", lambda c: dict(lengths=ints(2 ** 31 - 1, 17))),
             ("offsets that fall", lambda c: dict(new_offsets=ints(0, 3, 2))), ("offsets beyond the tokens", lambda c: dict(new_offsets=ints(0, 2, 2 ** 31 - 1))),
             ("offsets below zero", lambda c: dict(new_offsets=ints(-4, 2, 4))), ("offsets that start late", lambda c: dict(new_offsets=ints(1, 2, 4)))]
@@ -451,8 +455,9 @@ def _bad(device):
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("what", range(10))
 @pytest.mark.parametrize("most", [None, 2])
-def test_bad_values_are_reported_and_touch_nothing(device, what, most):
-    c = Paged([(20, 2), (17, 2)], 2, 2, 64, 16, device, garbage=7.0).fill()
+@pytest.mark.parametrize("wide", [3, 5000])
+def test_bad_values_are_reported_and_touch_nothing(device, what, most, wide):
+    c = Paged([(20, 2), (17, 2)], 2, 2, 64, 16, device, garbage=7.0, wide=wide).fill()
     change = _bad(device)[what][1](c)
     a = dict(k_pages=c.k, v_pages=c.v, page_table=c.table, new_offsets=c.offsets, lengths=c.lengths)
     a.update(change)
