@@ -15,8 +15,8 @@ namespace {
 typedef __nv_bfloat16 bf16;
 
 constexpr int kAppendThreads = 256;  // of a block, at most
-// Tokens of a block, where there are many.  16384 tokens, 32 heads and 8 kv heads of 128 (us): 68.0 with 2, 68.5 with 4, 94 with 8;
-// 33 prompts of up to 900, 12 heads of 64, with the norm: 32.1, 32.7, 44
+// Tokens of a block, where there are many.  16384 tokens, 32 heads and 8 kv heads of 128 (us): 68 with 2, 68.5 with 4, 94 with 8;
+// 33 prompts of up to 900, 12 heads of 64, with the norm: 32, 33, 44
 constexpr int kAppendTokens = 2;
 
 // eight values as four pairs of fp32
@@ -48,9 +48,10 @@ __device__ __forceinline__ void load8(const T* p, f32x2 (&f)[4]) {
 // HD / 16 lanes share a row (one head of one token): eight pairs each, 16 bytes from either half of the head.  A block takes T tokens
 // and as many of their rows as it has threads for, every thread the same row of each token, so that its addresses move on by one
 // stride.  Bound by memory: all loads of a thread are under way before it looks up where the rows go, and two fp32 operations go in one
-// instruction, as with single ones the issue slots were half full.
+// instruction, as with single ones the issue slots were half full.  Six blocks of 256 threads an SM: 30 and 67 us for the two cases
+// below, 33 and 72 with the registers that the compiler would take.
 template <int HD, int T, typename Table>
-__global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const PagedAppend p) {
+__global__ void __launch_bounds__(kAppendThreads, T == 1 ? 1 : 6) paged_append_kernel(const PagedAppend p) {
   constexpr int HALF = HD / 2, LPR = HD / 16;
   __shared__ long long k_at[T], v_at[T];  // of a token's rows in the pages; -1: it has none
   __shared__ int position[T];
