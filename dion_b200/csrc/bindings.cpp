@@ -1350,8 +1350,8 @@ __nv_bfloat16* bf16_data_out(const Tensor& t) { return reinterpret_cast<__nv_bfl
 
 // [tokens, heads, head_dim] with 16-byte rows; others are copied
 Tensor with_rows(const Tensor& t) {
-  const bool fits = on_16_bytes(t) && t.stride(2) == 1 && (t.size(0) == 1 || t.stride(0) % 8 == 0) &&
-                    (t.size(1) == 1 || t.stride(1) % 8 == 0);
+  bool fits = on_16_bytes(t) && t.stride(2) == 1;
+  for (int i = 0; i < 2; ++i) fits = fits && (t.size(i) == 1 || (t.stride(i) > 0 && t.stride(i) % 8 == 0));
   return fits ? t : t.clone(at::MemoryFormat::Contiguous);
 }
 

@@ -48,8 +48,8 @@ __device__ __forceinline__ void load8(const T* p, f32x2 (&f)[4]) {
 // HD / 16 lanes share a row (one head of one token): eight pairs each, 16 bytes from either half of the head.  A block takes T tokens
 // and as many of their rows as it has threads for, every thread the same row of each token, so that its addresses move on by one
 // stride.  Bound by memory: all loads of a thread are under way before it looks up where the rows go, and two fp32 operations go in one
-// instruction, as with single ones the issue slots were half full.  Six blocks of 256 threads an SM: 30 and 67 us for the two cases
-// below, 33 and 72 with the registers that the compiler would take.
+// instruction, as with single ones the issue slots were half full.  Six blocks of 256 threads an SM: 67 and 30 us for
+// the cases at kAppendTokens, 72 and 33 with the registers that the compiler would take.
 template <int HD, int T, typename Table>
 __global__ void __launch_bounds__(kAppendThreads, T == 1 ? 1 : 6) paged_append_kernel(const PagedAppend p) {
   constexpr int HALF = HD / 2, LPR = HD / 16;

@@ -33,17 +33,19 @@ constexpr int kShareCost = 64;
 // How rows are put together: `group` query heads of one kv head (`subs` such groups make all of its heads, where these are more than
 // a tile has rows) times `tokens` tokens are one tile of `height` rows, `tiles` of which go together.
 struct Tiling {
-  int height, tiles, group, subs, heads, tokens;  // heads: kv heads x subs; tokens: of all `tiles`
+  int height, tiles, group, subs, heads;          // heads: kv heads x subs
+  int per, tokens, all;                           // tokens of a tile and of all `tiles`; query heads of a kv head
   int fixed;                                      // what such rows cost apart from their keys, in keys
   int side = 1;                                   // heads that CTAs next to one another have, see Walk
   FastDiv by_group;
   Tiling() = default;
   Tiling(const PagedAttention& p, int height_, int tiles_, int fixed_) : height(height_), tiles(tiles_), fixed(fixed_) {
-    const int all = p.heads / p.kv_heads;
+    all = p.heads / p.kv_heads;
     subs = (all + height - 1) / height;
     group = (all + subs - 1) / subs;
     heads = p.kv_heads * subs;
-    tokens = height / group * tiles;
+    per = height / group;
+    tokens = per * tiles;
     by_group = FastDiv(group);
   }
 };
@@ -1229,31 +1231,46 @@ bool queries_tmap(CUtensorMap* map, const PagedAttention& p, int head_dim, const
 // caller knows less.
 struct Plan {
   Tiling tl;
+  bool many = false;  // rows for the tcgen05 kernel
   int ctas, cluster = 0, items = 0;  // cluster > 0: CTAs of an item, and the items that a sequence and head can have
   Plan(const PagedAttention& p, int head_dim) {
-    const long long group = p.heads / p.kv_heads, typical = (2ll * p.tokens + p.seqs - 1) / p.seqs;
-    const long long rows = std::min<long long>(p.max_new, typical) * group;
+    const long long group = p.heads / p.kv_heads, typical = std::min<long long>(p.max_new, (2ll * p.tokens + p.seqs - 1) / p.seqs);
+    const long long rows = typical * group, keys = (long long)p.max_pages << p.page_shift;
     const int sms = attn_grid(1 << 20);
-    tl = rows <= 64 ? Tiling(p, rows <= 16 ? 16 : rows <= 32 ? 32 : 64, 1, kRowsFixed) : Tiling(p, kBM, 2, kChunkFixed);
-    ctas = sms * (tl.tiles == 1 ? 2 : 1);
-    for (int h = 1; h <= tl.heads && h <= ctas; ++h)
-      if (tl.heads % h == 0 && ctas % h == 0) tl.side = h;
-    if (tl.tiles > 1) return;
-    // An item per cluster, without a second kernel, where the keys of its CTAs are few even if a sequence fills its row of the
-    // page table, which is all that the host knows: at most 4096 each, or 1024 where the clusters leave half of the SMs idle.  Both ways
-    // (us, shares / clusters; 32 heads on 8 of 128): one token over 1000 keys 12.0 / 6.9, over 4000 13.7 / 9.0, over 16000 17.5 / 20.5;
-    // 8 of 8000 52.0 / 44.7, 32 of up to 4000 54.2 / 48.2, 64 of 1000 54.7 / 46.0, 64 of 4000 165.7 / 149.5; of 8000 keys a CTA 40 items
-    // 201 / 227, 64 of up to 8000 138 / 131.
-    const long long most = (p.max_new + tl.tokens - 1) / tl.tokens, all = (long long)p.seqs * tl.heads * most;
-    const long long keys = (long long)p.max_pages << p.page_shift, slots = (long long)sms * (head_dim == 64 ? 3 : 2);
-    for (int c = kFewCluster; c >= 1; c /= 2) {
-      if (c > 1 ? all * c > slots : all > kFewItems) continue;
-      if (keys <= c * (2 * all * c < slots ? 1024ll : 4096ll)) {
-        cluster = c;
-        items = (int)most;
-        ctas = (int)all * c;
+    if (group <= 64) {
+      tl = Tiling(p, rows <= 16 ? 16 : rows <= 32 ? 32 : 64, 1, kRowsFixed);
+      // An item per cluster, without a second kernel, where the keys of its CTAs are few even if a sequence fills its row of the
+      // page table, which is all that the host knows: at most 4096 each, or 1024 where the clusters leave half of the SMs idle.  Both ways
+      // (us, shares / clusters; 32 heads on 8 of 128): one token over 1000 keys 12.0 / 6.9, over 4000 13.7 / 9.0, over 16000 17.5 / 20.5;
+      // 8 of 8000 52.0 / 44.7, 32 of up to 4000 54.2 / 48.2, 64 of 1000 54.7 / 46.0, 64 of 4000 165.7 / 149.5; of 8000 keys a CTA 40 items
+      // 201 / 227, 64 of up to 8000 138 / 131.
+      const long long most = (p.max_new + tl.per - 1) / tl.per, all = (long long)p.seqs * tl.heads * most;
+      const long long slots = (long long)sms * (head_dim == 64 && tl.height < 64 ? 3 : 2);
+      const long long likely = (long long)p.seqs * tl.heads * ((typical + tl.per - 1) / tl.per);
+      // More rows are better off there too while there is little work, at most 40 (20 of heads of 128) blocks of 64 rows by 64 keys per
+      // SM.  tcgen05 kernel / clusters (us): 12 heads of 64, 1 x 100 tokens 14.8 / 9.2, 4 x 300 24.8 / 9.3 (8 blocks), 8 x 500 32.6 / 26.6
+      // (41), 24 x 200 after 500 47.2 / 57.7 (86); 32 heads on 8 of 128, 1 x 400 25.2 / 14.8 (9.5), 1 x 700 34.3 / 26.6 (26), 1 x 200 after
+      // 3000 40.7 / 52.8 (35).
+      if (rows <= 64 || likely * ((keys + kKeys - 1) / kKeys) <= sms * 2560ll / head_dim) {
+        for (int c = kFewCluster; c >= 1; c /= 2) {
+          if (c > 1 ? all * c > slots || keys <= c * (kKeys / 2) : all > kFewItems) continue;
+          if (keys <= c * (2 * all * c < slots ? 1024ll : 4096ll)) {
+            cluster = c;
+            items = (int)most;
+            ctas = (int)all * c;
+          }
+          break;
+        }
       }
-      break;
+    }
+    if (cluster == 0 && rows > 64) {
+      many = true;
+      tl = Tiling(p, kBM, 2, kChunkFixed);
+    }
+    if (cluster == 0) {
+      ctas = sms * (many ? 1 : 2);
+      for (int h = 1; h <= tl.heads && h <= ctas; ++h)
+        if (tl.heads % h == 0 && ctas % h == 0) tl.side = h;
     }
   }
   int rows() const { return tl.height * tl.tiles; }
@@ -1313,11 +1330,11 @@ cudaError_t attention_launch(const PagedAttention& p, void* work, int* launches,
   parts.acc = reinterpret_cast<float*>(work);
   parts.ml = reinterpret_cast<float2*>(parts.acc + 2ll * plan.ctas * plan.rows() * D);
   parts.share = reinterpret_cast<Share*>(parts.ml + 2ll * plan.ctas * plan.rows());
-  const cudaError_t e = plan.tl.tiles == 1 ? rows_launch_d<D, false>(p, parts, plan, stream) : chunk_launch<D>(p, parts, plan, stream);
+  const cudaError_t e = !plan.many ? rows_launch_d<D, false>(p, parts, plan, stream) : chunk_launch<D>(p, parts, plan, stream);
   if (e != cudaSuccess) return e;
   // of a tile's rows those that a sequence can have
   const long long most = std::min<long long>(plan.rows(), (long long)p.max_new * (p.heads / p.kv_heads));
-  if (plan.tl.tiles == 1)
+  if (!plan.many)
     return launch_pdl(paged_join_kernel<D, 4, 1>, dim3(plan.ctas, (unsigned)std::min<long long>(most, 16)), dim3(128), 0, stream, 0, p, parts, plan.tl);
   return launch_pdl(paged_join_kernel<D, 1, 8>, dim3(plan.ctas, 16), dim3(256), 0, stream, 0, p, parts, plan.tl);
 }

@@ -175,12 +175,13 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     themselves: ``softmax(scale q K^T) V`` per head, ``[tokens, heads, head_dim]``.  `lengths` is what it was for ``paged_append``:
     without the new tokens.  Grouped heads: the kv heads divide the heads.  `scale` defaults to ``1 / sqrt(head_dim)``.
 
-    `max_new`: the most new tokens of a sequence, where the host knows it; a longer sequence is an error.  With 1 (a token each) or
-    a few the kernel for long chunks is not launched."""
+    `max_new`: the most new tokens of a sequence, where the host knows it; a longer sequence is an error.  It goes into the choice
+    of the kernel, as does the width of the page table, which says how long a sequence can be; any choice gives the result, to its
+    roundings."""
     _no_gradients("paged_attention", q, k_pages, v_pages)
     scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else float(scale)
-    if not 0.0 < scale < math.inf:
-        raise ValueError(f"paged_attention: the scale is positive and finite, not {scale}")
+    if not 2.0 ** -100 <= scale <= 2.0 ** 100:
+        raise ValueError(f"paged_attention: the scale is positive, from 2^-100 to 2^100, not {scale}")
     if max_new is None:
         max_new = q.shape[0]
     elif max_new < 1:

@@ -243,7 +243,7 @@ def test_attention_of_large_and_small_scores(device, new, wide):
 def test_attention_takes_scale_and_strided_queries(device):
     c = Paged([(50, 3), (0, 200)], 4, 4, 64, 16, device).fill()
     wide = torch.randn(c.tokens, 8, 64, device=device).bfloat16()
-    for q in (wide[:, ::2], wide[:, 4:], wide.transpose(0, 1).contiguous().transpose(0, 1)[:, :4], wide.repeat(1, 1, 2)[:, 1:5, 1:65]):
+    for q in (wide[:, ::2], wide[:, 4:], wide[:, :1].expand(-1, 4, -1), wide[:1, :4].expand(c.tokens, -1, -1), wide.transpose(0, 1).contiguous().transpose(0, 1)[:, :4], wide.repeat(1, 1, 2)[:, 1:5, 1:65]):
         _check_attention(ops.paged_attention(q, *c.where(), scale=0.3), q, c, 0.3)
 
 
@@ -399,7 +399,7 @@ def test_refusals_of_shapes_and_types(device):
                     dict(lengths=c.lengths.float()), dict(lengths=c.lengths[None]), dict(new_offsets=c.offsets.long())):
         with pytest.raises(ValueError):
             _call(c, q, **changes)
-    for changes in (dict(scale=0.0), dict(scale=-1.0), dict(scale=math.nan), dict(scale=math.inf), dict(max_new=0)):
+    for changes in (dict(scale=0.0), dict(scale=-1.0), dict(scale=math.nan), dict(scale=math.inf), dict(scale=1e-40), dict(scale=1e40), dict(max_new=0)):
         with pytest.raises(ValueError):
             ops.paged_attention(q, *c.where(), **changes)
     k = v = q[:, :2]
