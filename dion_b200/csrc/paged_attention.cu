@@ -680,21 +680,10 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
   }
 }
 
-// Joins the parts of items that several CTAs had and sees to nobody's rows.  Block (c, y) has the item that CTA c began, and of its
-// rows as many at a time as it has groups of WPR warps; the warps of a group share the parts.  Few rows come in many parts (a cache of
-// 4000 keys over the whole GPU in 30), so four warps take a row together there; many rows come in two or three, and a warp takes
-// each.  Bound by latency: what the next step needs is loaded before this one has decided whether, and the code is kept short, as
-// every call fetches it anew.
-template <int D, int WPR, int ROWS>
-__global__ void __launch_bounds__(32 * WPR * ROWS) paged_join_kernel(const PagedAttention p, const Parts parts, const __grid_constant__ Tiling tl) {
-  constexpr int E = D / 32, AT_ONCE = WPR > 1 ? 4 : 2;  // columns of a lane, parts whose loads are under way at once
-  __shared__ float sums[WPR][D + 2];
-  pdl_trigger();
-  pdl_wait();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = blockIdx.x, ctas = gridDim.x, rows = tl.height * tl.tiles;
-  const int side = tl.side;  // CTAs c, c + side ... have the item's parts
-  const Share mine = parts.share[c];
-  int last = 0;  // how many of them until the one that ends it
+// CTAs c, c + side ... have the parts of the item that CTA c has begun: how many come after c, up to the one that ends it.  By a whole
+// warp; any answer, in bounds, where c has begun none.
+__device__ __forceinline__ int parts_after(const Parts& parts, const Share& mine, int c, int side, int ctas, int lane) {
+  int last = 0;
   for (bool more = true; more;) {
     const int i = c + (last + 1 + lane) * side;
     const Share s = parts.share[min(i, ctas - 1)];
@@ -702,20 +691,44 @@ __global__ void __launch_bounds__(32 * WPR * ROWS) paged_join_kernel(const Paged
     more = at == 0 && mine.b >= 0;
     last += more ? 32 : __ffs(at);
   }
-  last = min(last, (ctas - 1 - c) / side);
+  return min(last, (ctas - 1 - c) / side);
+}
+template <int E>
+__device__ __forceinline__ void load_columns(const float* from, float (&v)[E]) {
+  if constexpr (E == 4) {
+    const float4 x = *reinterpret_cast<const float4*>(from);
+    v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
+  } else {
+    const float2 x = *reinterpret_cast<const float2*>(from);
+    v[0] = x.x, v[1] = x.y;
+  }
+}
+
+// Joins the parts of items that several CTAs had and sees to nobody's rows; for few rows, which come in many parts (a cache of 4000
+// keys over the whole GPU in 30).  Block (c, y) has the item that CTA c began, and of its rows every gridDim.y-th, whose parts the
+// WARPS warps share.  Bound by latency: what the next step needs is loaded before this one has decided whether, and the code is
+// kept short, as every call fetches it anew.
+template <int D, int WARPS>
+__global__ void __launch_bounds__(32 * WARPS) paged_join_kernel(const PagedAttention p, const Parts parts, const __grid_constant__ Tiling tl) {
+  constexpr int E = D / 32;  // columns of a lane
+  __shared__ float sums[WARPS][D + 2];
+  pdl_trigger();
+  pdl_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = blockIdx.x, ctas = gridDim.x, rows = tl.height, side = tl.side;
+  const Share mine = parts.share[c];
+  const int last = parts_after(parts, mine, c, side, ctas, lane);
   if (mine.b >= 0) {
     const Sequence s = sequence(p, mine.b);
-    const int sub = warp % WPR;
-    for (int r = blockIdx.y * ROWS + warp / WPR; r < rows; r += ROWS * gridDim.y) {
+    for (int r = blockIdx.y; r < rows; r += gridDim.y) {
       int token, h;
-      if (!row_of(p, tl, s.n, mine.head, mine.item, r / tl.height, r % tl.height, token, h)) continue;  // all warps of the row
+      if (!row_of(p, tl, s.n, mine.head, mine.item, 0, r, token, h)) continue;  // the whole block
       float top = -INFINITY, sum = 0.f, acc[E];
 #pragma unroll
       for (int e = 0; e < E; ++e) acc[e] = 0.f;
       auto slot = [&](int nth) { return (2 * (c + (long long)nth * side) + (nth == 0 ? 1 : 0)) * rows + r; };
-      // this warp's parts are numbers sub, sub + WPR ..., 32 at a time
-      for (int base = sub; base <= last; base += 32 * WPR) {
-        const int nth = base + lane * WPR, n = min(32, (last - base) / WPR + 1);
+      // this warp's parts are numbers warp, warp + WARPS ..., 32 at a time
+      for (int base = warp; base <= last; base += 32 * WARPS) {
+        const int nth = base + lane * WARPS, n = min(32, (last - base) / WARPS + 1);
         const float2 t = nth <= last ? parts.ml[slot(nth)] : make_float2(-INFINITY, 0.f);
         float most = t.x;
 #pragma unroll
@@ -726,21 +739,12 @@ __global__ void __launch_bounds__(32 * WPR * ROWS) paged_join_kernel(const Paged
 #pragma unroll
         for (int e = 0; e < E; ++e) acc[e] *= f;
 #pragma unroll 1
-        for (int k = 0; k < n; k += AT_ONCE) {
-          float v[AT_ONCE][E];
+        for (int k = 0; k < n; k += 4) {
+          float v[4][E];
 #pragma unroll
-          for (int j = 0; j < AT_ONCE; ++j) {
-            const float* from = parts.acc + slot(base + min(k + j, n - 1) * WPR) * D + lane * E;
-            if constexpr (E == 4) {
-              const float4 x = *reinterpret_cast<const float4*>(from);
-              v[j][0] = x.x, v[j][1] = x.y, v[j][2] = x.z, v[j][3] = x.w;
-            } else {
-              const float2 x = *reinterpret_cast<const float2*>(from);
-              v[j][0] = x.x, v[j][1] = x.y;
-            }
-          }
+          for (int j = 0; j < 4; ++j) load_columns<E>(parts.acc + slot(base + min(k + j, n - 1) * WARPS) * D + lane * E, v[j]);
 #pragma unroll
-          for (int j = 0; j < AT_ONCE; ++j) {
+          for (int j = 0; j < 4; ++j) {
             const float wj = __shfl_sync(0xffffffffu, w, (k + j) & 31);
             if (k + j < n && wj > 0.f) {  // a part that saw none of the row's keys has nothing written
 #pragma unroll
@@ -751,36 +755,106 @@ __global__ void __launch_bounds__(32 * WPR * ROWS) paged_join_kernel(const Paged
       }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      if constexpr (WPR > 1) {
-        if (lane == 0) sums[sub][D] = top, sums[sub][D + 1] = sum;
+      if (lane == 0) sums[warp][D] = top, sums[warp][D + 1] = sum;
 #pragma unroll
-        for (int e = 0; e < E; ++e) sums[sub][lane * E + e] = acc[e];
-        __syncthreads();
+      for (int e = 0; e < E; ++e) sums[warp][lane * E + e] = acc[e];
+      __syncthreads();
+      if (warp == 0) {
         const float mine_top = top;
 #pragma unroll 1
-        for (int i = 0; i < WPR; ++i) top = fmaxf(top, sums[i][D]);
+        for (int i = 1; i < WARPS; ++i) top = fmaxf(top, sums[i][D]);
         float f = fast_exp2(mine_top - top);
         sum *= f;
 #pragma unroll
         for (int e = 0; e < E; ++e) acc[e] *= f;
 #pragma unroll 1
-        for (int i = 1; i < WPR; ++i) {  // only the first warp's result counts
+        for (int i = 1; i < WARPS; ++i) {
           f = fast_exp2(sums[i][D] - top);
           sum += sums[i][D + 1] * f;
 #pragma unroll
           for (int e = 0; e < E; ++e) acc[e] += sums[i][lane * E + e] * f;
         }
-      }
-      if (sub == 0) {
         const float inv = sum > 0.f ? 1.f / sum : 0.f;
         bf16* dst = p.out + ((long long)(s.first + token) * p.heads + h) * D + lane * E;
 #pragma unroll
         for (int e = 0; e < E; e += 2) *reinterpret_cast<uint32_t*>(dst + e) = pack_bf16x2(acc[e] * inv, acc[e + 1] * inv);
       }
-      if constexpr (WPR > 1) __syncthreads();
+      __syncthreads();
     }
   }
-  if (blockIdx.y == 0) nobodys_rows<D>(p, c, ctas, threadIdx.x, 32 * WPR * ROWS);
+  if (blockIdx.y == 0) nobodys_rows<D>(p, c, ctas, threadIdx.x, 32 * WARPS);
+}
+
+// The same for many rows, which come in two or three parts: a warp takes four rows at a time, their maxima and sums of up to eight
+// parts in one load, so that they are all under way at once.  With the kernel above it, 2048 tokens over 6000 cached, two sequences, 32
+// heads on 8 of 128, take 415 us, 421 with a row after the other; with blocks of eight warps instead of four a call that has nothing
+// to join took 227 us instead of 208.
+constexpr int kJoinWarps = 4, kJoinRows = 4;
+template <int D>
+__global__ void __launch_bounds__(32 * kJoinWarps) paged_join_many_kernel(const PagedAttention p, const Parts parts, const __grid_constant__ Tiling tl) {
+  constexpr int E = D / 32, R = kJoinRows, K = 32 / R;  // columns of a lane, rows of a warp, parts at a time
+  pdl_trigger();
+  pdl_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = blockIdx.x, ctas = gridDim.x, rows = tl.height * tl.tiles, side = tl.side;
+  const Share mine = parts.share[c];
+  const int last = parts_after(parts, mine, c, side, ctas, lane);
+  if (mine.b >= 0) {
+    const Sequence s = sequence(p, mine.b);
+    for (int r0 = (blockIdx.y * kJoinWarps + warp) * R; r0 < rows; r0 += gridDim.y * kJoinWarps * R) {
+      auto slot = [&](int nth) { return (2 * (c + (long long)nth * side) + (nth == 0 ? 1 : 0)) * rows + r0; };
+      float top = -INFINITY, sum = 0.f, acc[R][E];  // top and sum of row r0 + lane / K, this lane's parts
+#pragma unroll
+      for (int j = 0; j < R; ++j)
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[j][e] = 0.f;
+      for (int base = 0; base <= last; base += K) {
+        const int nth = base + lane % K, n = min(K, last - base + 1);
+        const float2 t = nth <= last ? parts.ml[slot(nth) + lane / K] : make_float2(-INFINITY, 0.f);
+        float most = t.x;
+#pragma unroll
+        for (int o = K / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+        const float top2 = fmaxf(top, most), neg = top2 == -INFINITY ? 0.f : -top2, f = fast_exp2(top + neg), w = fast_exp2(t.x + neg);
+        sum = sum * f + t.y * w;
+        top = top2;
+        if (base > 0) {
+#pragma unroll
+          for (int j = 0; j < R; ++j) {
+            const float fj = __shfl_sync(0xffffffffu, f, j * K);
+#pragma unroll
+            for (int e = 0; e < E; ++e) acc[j][e] *= fj;
+          }
+        }
+#pragma unroll 2
+        for (int k = 0; k < n; ++k) {
+          float v[R][E];
+#pragma unroll
+          for (int j = 0; j < R; ++j) load_columns<E>(parts.acc + (slot(base + k) + j) * D + lane * E, v[j]);
+#pragma unroll
+          for (int j = 0; j < R; ++j) {
+            const float wj = __shfl_sync(0xffffffffu, w, j * K + k);
+            if (wj > 0.f) {  // a part that saw none of the row's keys has nothing written
+#pragma unroll
+              for (int e = 0; e < E; ++e) acc[j][e] += wj * v[j][e];
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int o = K / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      const float inv = sum > 0.f ? 1.f / sum : 0.f;
+#pragma unroll
+      for (int j = 0; j < R; ++j) {
+        const int r = r0 + j;
+        const float f = __shfl_sync(0xffffffffu, inv, j * K);
+        int token, h;
+        if (!row_of(p, tl, s.n, mine.head, mine.item, r / kBM, r % kBM, token, h)) continue;
+        bf16* dst = p.out + ((long long)(s.first + token) * p.heads + h) * D + lane * E;
+#pragma unroll
+        for (int e = 0; e < E; e += 2) *reinterpret_cast<uint32_t*>(dst + e) = pack_bf16x2(acc[j][e] * f, acc[j][e + 1] * f);
+      }
+    }
+  }
+  if (blockIdx.y == 0) nobodys_rows<D>(p, c, ctas, threadIdx.x, 32 * kJoinWarps);
 }
 
 // ---------------------------------------------------------------------------------- many rows: tcgen05
@@ -1335,8 +1409,9 @@ cudaError_t attention_launch(const PagedAttention& p, void* work, int* launches,
   // of a tile's rows those that a sequence can have
   const long long most = std::min<long long>(plan.rows(), (long long)p.max_new * (p.heads / p.kv_heads));
   if (!plan.many)
-    return launch_pdl(paged_join_kernel<D, 4, 1>, dim3(plan.ctas, (unsigned)std::min<long long>(most, 16)), dim3(128), 0, stream, 0, p, parts, plan.tl);
-  return launch_pdl(paged_join_kernel<D, 1, 8>, dim3(plan.ctas, 16), dim3(256), 0, stream, 0, p, parts, plan.tl);
+    return launch_pdl(paged_join_kernel<D, 4>, dim3(plan.ctas, (unsigned)std::min<long long>(most, 16)), dim3(128), 0, stream, 0, p, parts, plan.tl);
+  return launch_pdl(paged_join_many_kernel<D>, dim3(plan.ctas, plan.rows() / (kJoinWarps * kJoinRows)), dim3(32 * kJoinWarps), 0, stream, 0, p, parts,
+                    plan.tl);
 }
 
 }  // namespace
