@@ -1,6 +1,7 @@
 // torch bindings for the sm_100a kernels of dion_b200.  Registered as
 // torch.ops.dion_b200.* by loading the shared library; no Python C-API use.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/library.h>
 #include <torch/torch.h>
@@ -1294,6 +1295,23 @@ void symm_reduce_scatter(const Tensor& inp, Tensor out, at::IntArrayRef peers, i
 
 
 // ----------------------------------------------------------------------------- paged cache
+// These run once a layer and sampled token, where the host's part is longer than the kernel's (append of one token 2.8 us, its call 9):
+// what would be Python in front of the call is decided here.
+
+// The operators have no gradient.
+void refuse_gradients(const char* name, std::initializer_list<const Tensor*> tensors) {
+  if (!at::GradMode::is_enabled()) return;
+  for (const Tensor* t : tensors)
+    TORCH_CHECK(!t->defined() || !t->requires_grad(), name, " has no gradient: call it under torch.no_grad() or with detached inputs");
+}
+// Types and head dimensions that the kernels take; others go the plain way.
+bool paged_on_kernels(const Tensor& q) {
+  return q.scalar_type() == at::kBFloat16 && q.dim() > 0 && (q.size(-1) == 64 || q.size(-1) == 128);
+}
+// at::empty without the way through the dispatcher
+Tensor empty_like_of(at::IntArrayRef sizes, const Tensor& t) {
+  return at::detail::empty_cuda(sizes, t.scalar_type(), t.device(), std::nullopt);
+}
 
 // Pages [pages, page_size, kv heads, head_dim] in any order that TMA and 16-byte accesses can take, with the table, offsets
 // and lengths of the sequences whose new tokens the rows of q are.  Sets what the two structs name alike.
@@ -1355,9 +1373,12 @@ Tensor with_rows(const Tensor& t) {
   return fits ? t : t.clone(at::MemoryFormat::Contiguous);
 }
 
-Tensor paged_append(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& cos_, const Tensor& sin_, Tensor k_pages,
+std::optional<Tensor> paged_append(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& cos_, const Tensor& sin_, Tensor k_pages,
                     Tensor v_pages, const Tensor& page_table, const Tensor& offsets, const Tensor& lengths, double eps,
                     Tensor status) {
+  refuse_gradients("paged_append", {&q_, &k_, &v_, &k_pages, &v_pages});
+  if (!paged_on_kernels(q_)) return std::nullopt;
+  TORCH_CHECK_VALUE(!(eps < 0.) || eps == -1., "paged_append: norm_eps is None or not negative, not ", eps);
   dion::PagedAppend p;
   const c10::cuda::CUDAGuard guard(q_.device());
   describe_paged(p, "paged_append", q_, k_pages, v_pages, page_table, offsets, lengths, status);
@@ -1375,7 +1396,7 @@ Tensor paged_append(const Tensor& q_, const Tensor& k_, const Tensor& v_, const 
     return on_16_bytes(t) && t.stride(1) == 1 && t.stride(0) * t.element_size() % 16 == 0 ? t : t.clone(at::MemoryFormat::Contiguous);
   };
   const Tensor q = with_rows(q_), k = with_rows(k_), v = with_rows(v_), cos = table(cos_), sin = table(sin_);
-  Tensor out = at::empty({N, p.heads, D}, q.options());
+  Tensor out = empty_like_of({N, p.heads, D}, q);
   p.q = bf16_data(q), p.k = bf16_data(k), p.v = bf16_data(v);
   p.q_out = bf16_data_out(out), p.k_pages = bf16_data_out(k_pages), p.v_pages = bf16_data_out(v_pages);
   p.cos = cos.data_ptr(), p.sin = sin.data_ptr();
@@ -1388,8 +1409,10 @@ Tensor paged_append(const Tensor& q_, const Tensor& k_, const Tensor& v_, const 
   return out;
 }
 
-Tensor paged_attention(const Tensor& q_, const Tensor& k_pages, const Tensor& v_pages, const Tensor& page_table,
+std::optional<Tensor> paged_attention(const Tensor& q_, const Tensor& k_pages, const Tensor& v_pages, const Tensor& page_table,
                        const Tensor& offsets, const Tensor& lengths, double scale, int64_t max_new, Tensor status) {
+  refuse_gradients("paged_attention", {&q_, &k_pages, &v_pages});
+  if (!paged_on_kernels(q_)) return std::nullopt;
   dion::PagedAttention p;
   const c10::cuda::CUDAGuard guard(q_.device());
   describe_paged(p, "paged_attention", q_, k_pages, v_pages, page_table, offsets, lengths, status);
@@ -1397,7 +1420,7 @@ Tensor paged_attention(const Tensor& q_, const Tensor& k_pages, const Tensor& v_
   if (N == 0 || p.seqs == 0) return at::zeros({N, p.heads, D}, q_.options());
   TORCH_CHECK_VALUE(p.pages > 0, "paged_attention: there are no pages");
   const Tensor q = with_rows(q_);
-  Tensor out = at::empty({N, p.heads, D}, q.options());
+  Tensor out = empty_like_of({N, p.heads, D}, q);
   p.q = bf16_data(q), p.k_pages = bf16_data(k_pages), p.v_pages = bf16_data(v_pages);
   p.out = bf16_data_out(out);
   p.q_token = q.stride(0), p.q_head = q.stride(1);
@@ -1414,6 +1437,8 @@ Tensor paged_attention(const Tensor& q_, const Tensor& k_pages, const Tensor& v_
 
 std::tuple<Tensor, Tensor> verify_drafts(const Tensor& target, const std::optional<Tensor>& draft, const Tensor& tokens,
                                          const Tensor& uniforms, Tensor status) {
+  refuse_gradients("verify_drafts", {&target, &uniforms});
+  if (draft.has_value()) refuse_gradients("verify_drafts", {&*draft});
   const c10::cuda::CUDAGuard guard(target.device());
   TORCH_CHECK_VALUE(target.dim() == 3 && target.size(1) >= 1 && target.size(2) >= 1 && target.scalar_type() == at::kFloat,
                     "verify_drafts: the target's probabilities are fp32 [sequences, drafts + 1, vocabulary], not ", target.scalar_type(), " ", target.sizes());
@@ -1430,7 +1455,7 @@ std::tuple<Tensor, Tensor> verify_drafts(const Tensor& target, const std::option
                     "verify_drafts: tensors on one device");
   TORCH_CHECK_VALUE(V < (1ll << 31) - (1 << 16) && B < (1 << 28) && K < (1ll << 31) - 64,
                     "verify_drafts: more sequences, drafts or tokens of the vocabulary than 32-bit indices take");
-  Tensor accepted = at::empty({B}, tokens.options()), token = at::empty({B}, tokens.options());
+  Tensor accepted = empty_like_of({B}, tokens), token = empty_like_of({B}, tokens);
   if (B == 0) return {accepted, token};
   auto rows = [](const Tensor& t) { return t.stride(-1) == 1 || t.size(-1) <= 1 ? t : t.contiguous(); };
   const Tensor t = rows(target), x = rows(tokens), u = rows(uniforms);
@@ -1545,10 +1570,10 @@ TORCH_LIBRARY(dion_b200, m) {
   m.def("dion_q_norm(Tensor R32, Tensor ss, Tensor Qm, float eps, Tensor(a!)? Qn, Tensor(b!)? Qs, int qs_col0) -> ()");
   m.def(
       "paged_append(Tensor q, Tensor k, Tensor v, Tensor cos, Tensor sin, Tensor(a!) k_pages, Tensor(b!) v_pages, "
-      "Tensor page_table, Tensor new_offsets, Tensor lengths, float eps, Tensor(c!) status) -> Tensor");
+      "Tensor page_table, Tensor new_offsets, Tensor lengths, float eps, Tensor(c!) status) -> Tensor?");
   m.def(
       "paged_attention(Tensor q, Tensor k_pages, Tensor v_pages, Tensor page_table, Tensor new_offsets, Tensor lengths, "
-      "float scale, int max_new, Tensor(a!) status) -> Tensor");
+      "float scale, int max_new, Tensor(a!) status) -> Tensor?");
   m.def(
       "verify_drafts(Tensor target, Tensor? draft, Tensor tokens, Tensor uniforms, Tensor(a!) status) -> (Tensor, Tensor)");
   m.def("launch_count() -> int", &launch_count);

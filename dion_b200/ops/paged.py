@@ -34,11 +34,15 @@ def _no_gradients(name: str, *tensors: Optional[torch.Tensor]) -> None:
             raise RuntimeError(f"{name} has no gradient: call it under torch.no_grad() or with detached inputs")
 
 
-def _on_kernels(q: torch.Tensor) -> bool:
-    return q.is_cuda and q.dtype is torch.bfloat16 and q.shape[-1] in (64, 128) and runtime.use_cuda_kernels(q)
+_kernels = None  # the operators of the library, from the first call with CUDA tensors on
 
 
-_OPS = torch.ops.dion_b200  # the operators are looked up on it at the first call, when the library has been loaded
+def _load(t: torch.Tensor):
+    global _kernels
+    runtime.use_cuda_kernels(t)
+    lib = torch.ops.dion_b200
+    _kernels = (lib.paged_append.default, lib.paged_attention.default, lib.verify_drafts.default)
+    return _kernels
 
 
 # --------------------------------------------------------------------------- plain path
@@ -159,12 +163,14 @@ def paged_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.T
     pages in place and returns the rotated q.  ``cos`` / ``sin``: ``[positions, head_dim / 2]``, bf16 or fp32, as
     ``rotary_tables`` makes them.  With `norm_eps` every head of q and k goes through an RMS norm after the rotation, as
     ``rope_qknorm`` does; without, this is ``rope``.  fp32 arithmetic, rounded once."""
-    _no_gradients("paged_append", q, k, v, k_pages, v_pages)
     if norm_eps is not None and not norm_eps >= 0.0:
         raise ValueError(f"paged_append: norm_eps is None or not negative, not {norm_eps}")
-    if _on_kernels(q):
-        return _OPS.paged_append(q, k, v, cos, sin, k_pages, v_pages, page_table, new_offsets, lengths,
-                                 -1.0 if norm_eps is None else norm_eps, runtime.status_tensor(q.device))
+    if q.is_cuda:
+        out = (_kernels or _load(q))[0](q, k, v, cos, sin, k_pages, v_pages, page_table, new_offsets, lengths,
+                                        -1.0 if norm_eps is None else norm_eps, runtime.status_tensor(q.device))
+        if out is not None:
+            return out
+    _no_gradients("paged_append", q, k, v, k_pages, v_pages)
     return _append_plain(q, k, v, cos, sin, k_pages, v_pages, page_table, new_offsets, lengths, norm_eps)
 
 
@@ -178,17 +184,18 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     `max_new`: the most new tokens of a sequence, where the host knows it; a longer sequence is an error.  It goes into the choice
     of the kernel, as does the width of the page table, which says how long a sequence can be; any choice gives the result, to its
     roundings."""
-    _no_gradients("paged_attention", q, k_pages, v_pages)
-    scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else float(scale)
+    scale = 1.0 / math.sqrt(q.size(-1)) if scale is None else float(scale)
     if not 2.0 ** -100 <= scale <= 2.0 ** 100:
         raise ValueError(f"paged_attention: the scale is positive, from 2^-100 to 2^100, not {scale}")
     if max_new is None:
-        max_new = q.shape[0]
+        max_new = q.size(0)
     elif max_new < 1:
         raise ValueError(f"paged_attention: max_new is at least 1, not {max_new}")
-    if _on_kernels(q):
-        return _OPS.paged_attention(q, k_pages, v_pages, page_table, new_offsets, lengths, scale, max_new,
-                                    runtime.status_tensor(q.device))
+    if q.is_cuda:
+        out = (_kernels or _load(q))[1](q, k_pages, v_pages, page_table, new_offsets, lengths, scale, max_new, runtime.status_tensor(q.device))
+        if out is not None:
+            return out
+    _no_gradients("paged_attention", q, k_pages, v_pages)
     return _attention_plain(q, k_pages, v_pages, page_table, new_offsets, lengths, scale, max_new)
 
 
@@ -203,9 +210,9 @@ def verify_drafts(target_probs: torch.Tensor, draft_probs: Optional[torch.Tensor
     that fell, or from the target's row behind the last: the lowest token whose running sum exceeds u times the whole.  Sums are in
     64 bits.  Where p - q leaves nothing, p itself stands in; differences and probabilities that are negative, infinite or no
     numbers count as zero there, and a row of zeros gives token 0.  Returns ``(accepted, token)``, int64 per sequence."""
+    if target_probs.is_cuda:
+        return (_kernels or _load(target_probs))[2](target_probs, draft_probs, draft_tokens, uniforms, runtime.status_tensor(target_probs.device))
     _no_gradients("verify_drafts", target_probs, draft_probs, uniforms)
-    if target_probs.is_cuda and runtime.use_cuda_kernels(target_probs):
-        return _OPS.verify_drafts(target_probs, draft_probs, draft_tokens, uniforms, runtime.status_tensor(target_probs.device))
     p, q = target_probs, draft_probs
 
     def need(ok, what):
