@@ -1,10 +1,12 @@
 // Causal attention of new tokens over a paged cache of keys and values:
 //   out = softmax(scale q K[0..p]^T) V[0..p],   p = lengths[b] + i of row i of sequence b.
 //
-// The rows of a sequence that share a kv head (new tokens x heads of its group, token by token) make one tile of queries.  The keys
-// are taken once per tile with the running maximum and sum of a softmax, and all keys of all tiles are dealt out evenly over the
-// CTAs, whatever the lengths: a CTA's share may end inside a tile, whose parts a second kernel then joins.  The shares follow from
-// the sizes alone, so a call gives the same bits every time.
+// The rows of a sequence that share a kv head (new tokens x heads of its group, token by token) make tiles of queries.  The keys
+// are taken once per tile with the running maximum and sum of a softmax.  Few rows are bound by the bandwidth of the cache and go
+// through mma.sync (paged_rows_kernel), many by the tensor core and the exponentials and go through tcgen05 (paged_chunk_kernel).
+// Either way all keys of all tiles are dealt out evenly over the CTAs, whatever the lengths: a CTA's share may end inside a tile,
+// whose parts a second kernel then joins.  Where the page table says that keys are few, a cluster of CTAs has a tile's instead and
+// joins them itself.  Who has what follows from the sizes alone, so a call gives the same bits every time.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <math.h>
@@ -326,7 +328,8 @@ __device__ __forceinline__ void nobodys_rows(const PagedAttention& p, int block,
 // Bound by the bandwidth of the cache: 64 keys are 32 KB (head dimension 128), which an SM gets in 1400 cycles, and take four
 // warps some 600.  So the legacy products, whose tiles are 16 rows high, do: the rows of single tokens fill no more.  A warp loads
 // 64 keys a stage by TMA, the boxes of several pages where they are smaller; where the rows fit one 16-row tile the four others
-// take 16 keys each and join their sums per item, else they share the keys and have rows of their own.
+// take 16 keys each and join their sums per item, else they share the keys and have rows of their own.  Two caches of 120000 keys, 8
+// kv heads of 128: 152 us, 6.4 TB/s; 64 of up to 8000 139 us, 6.1 TB/s.
 //
 // FEW: a cluster has one item, its CTAs equal parts of the keys, and the parts are joined over the cluster's shared memory.  That
 // saves the second kernel where items are short; what counts there is the chain of latencies.
@@ -889,6 +892,14 @@ __device__ __forceinline__ int tile_end(const Walk<kBM>& w, const Tiling& tl, in
 // a query row per thread and a warp that issues its products, so that one tile's exponentials run under the other's products.  K
 // and V come page by page; keys behind the last one are masked and their values, which may be no numbers, replaced by zeros in
 // shared memory by the softmax warps before they hand on the weights.
+//
+// A unit of 128 keys of both tiles takes 3200 cycles for heads of 64 and 4100 of 128 (2048 tokens over 6000 cached, two sequences, 32
+// heads on 8 of 128: 415 us, 1.13 PFLOP/s).  Its exponentials take 2048 of the special function unit, its products 1024 and 2048
+// of the tensor core; what is on top is the chain of a tile: at 128 its next S waits for P V, as P lies over S, 1700 cycles of
+// which 1024 are products, and at 64 both tiles' exponentials run at the same time.  Measured and not kept (cycles a unit, 64 / 128):
+// a quarter of the exponentials by a polynomial (3200 / 4700, the multiply-adds take 14 cycles a value of a warp, the special function
+// unit 8), two threads for a row (3400 / 5500), P V in two halves (3200 / 4800 with both tiles), the next scores
+// loaded during the exponentials (3400), two CTAs with a tile each (3400), a lock between the tiles' exponentials (3800 / 3600).
 template <int D>
 __global__ void __launch_bounds__(kChunkThreads, 1)
 paged_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,

@@ -91,7 +91,7 @@ def test_cached_passes_give_the_logits_of_whole_ones(make):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("make,kw", [(_gpt, dict(width=256, heads=4)), (_gpt, dict(width=256, heads=2)), (_llama, dict(width=256, heads=4, kv_heads=2))])
+@pytest.mark.parametrize("make,kw", [(_gpt, dict(width=256, heads=4)), (_gpt, dict(width=256, heads=2)), (_gpt, dict(width=256, heads=8)), (_llama, dict(width=256, heads=4, kv_heads=2))])
 def test_cached_passes_on_the_kernels(make, kw):
     """bf16 activations are rounded some ten times a layer on either way, each time by at most a half step: two layers and
     the head are within 21 half steps of the exact, and of one another within twice that, as norms."""

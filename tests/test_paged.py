@@ -260,20 +260,58 @@ def test_other_types_run_plainly_on_the_gpu():
     torch.testing.assert_close(ops.paged_attention(q, *c.where()).double(), _attend(q, c)[0], rtol=1e-4, atol=1e-5)
 
 
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("new,wide", [(1, 3), (1, 5000), (90, 5000)])
+def test_sequences_that_share_pages(device, new, wide):
+    """The pages of a common beginning stand in both sequences' tables; each goes on in pages of its own."""
+    c = Paged([(70, new), (64, new), (48, 0)], 4, 2, 64, 16, device, wide=wide).fill()
+    c.table[1, :3] = c.table[0, :3]
+    q = torch.randn(c.tokens, 4, 64, device=device).bfloat16()
+    _check_attention(ops.paged_attention(q, *c.where()), q, c)
+
+
 @pytest.mark.gpu
-def test_append_and_attention_in_a_graph_and_on_another_stream():
+def test_pages_beyond_32_bits():
+    """Pages of 2.6e9 values each: offsets that pass 2^31 values and 2^32 bytes, in both kernels and the append."""
+    pages, size, heads, dim = 40000, 64, 8, 128
+    c = Paged([(100, 1), (300, 40), (0, 200)], heads, heads, dim, size, "cpu")
+    c.k = c.v = None
+    c.k, c.v = (torch.empty(pages, size, heads, dim, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    c.table[c.table >= 0] += pages - 1 - int(c.table.max())
+    c.table, c.offsets, c.lengths = c.table.cuda(), c.offsets.cuda(), c.lengths.cuda()
+    c.fill(upto_new=False)
+    q, k, v = (torch.randn(c.tokens, heads, dim, device="cuda").bfloat16() for _ in range(3))
+    cos, sin = N.rotary_tables(512, dim, "cuda")
+    turned = ops.paged_append(q, k, v, cos, sin, *c.where())
+    ops.check_status()
+    for b, (p, n) in enumerate(c.sizes):
+        page, row = c.slots(b, p, p + n)
+        rows = slice(c.starts[b], c.starts[b] + n)
+        assert torch.equal(c.v[page, row], v[rows])
+        want, most = _turned(k[rows], cos[p:p + n], sin[p:p + n], None)
+        assert ((c.k[page, row].double() - want).abs() <= HALF_STEP * want.abs() + 16 * U32 * most).all()
+    for most in (None, 200):
+        _check_attention(ops.paged_attention(turned, *c.where(), max_new=most), turned, c)
+    c.table = torch.cat([c.table, torch.zeros(3, 5000, dtype=torch.int32, device="cuda")], 1)
+    _check_attention(ops.paged_attention(turned, *c.where()), turned, c)
+    ops.check_status()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new,wide", [(2, 8), (2, 5000), (90, 5000)])
+def test_append_and_attention_in_a_graph_and_on_another_stream(new, wide):
     """Captured once and replayed with other lengths, tables and inputs; two graphs in turn, on a stream of their own."""
-    sizes = [(40, 2), (300, 2), (0, 2)]
+    sizes = [(40, new), (300, new), (0, new)]
     cos, sin = N.rotary_tables(512, 64, "cuda")
     side = torch.cuda.Stream()
     graphs = []
     for k in range(2):
-        c = Paged([(p + 20 * k, n) for p, n in sizes], 8, 4, 64, 16, "cuda", wide=8).fill(upto_new=False)
+        c = Paged([(p + 20 * k, n) for p, n in sizes], 8, 4, 64, 16, "cuda", wide=wide).fill(upto_new=False)
         qkv = torch.randn(c.tokens, 16, 64, device="cuda").bfloat16()
 
         def call(c=c, qkv=qkv):
             q, k_, v = qkv.split([8, 4, 4], 1)
-            return ops.paged_attention(ops.paged_append(q, k_, v, cos, sin, *c.where(), norm_eps=1e-6), *c.where(), max_new=2)
+            return ops.paged_attention(ops.paged_append(q, k_, v, cos, sin, *c.where(), norm_eps=1e-6), *c.where(), max_new=new)
 
         side.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(side):
