@@ -613,7 +613,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             if (to[i] < 0) continue;
-            const float inv = l[i] > 0.f ? 1.f / l[i] : 0.f;
+            const float inv = 1.f / l[i];  // the row sees a key; no numbers, or none but -infinity, stay no numbers
 #pragma unroll
             for (int c = 0; c < D / 8; ++c)
               *reinterpret_cast<uint32_t*>(p.out + to[i] + c * 8 + pair) = pack_bf16x2(o[c][2 * i] * inv, o[c][2 * i + 1] * inv);
@@ -777,7 +777,7 @@ __global__ void __launch_bounds__(32 * WARPS) paged_join_kernel(const PagedAtten
 #pragma unroll
           for (int e = 0; e < E; ++e) acc[e] += sums[i][lane * E + e] * f;
         }
-        const float inv = sum > 0.f ? 1.f / sum : 0.f;
+        const float inv = 1.f / sum;  // no number where a part's sum is none, whatever its weight
         bf16* dst = p.out + ((long long)(s.first + token) * p.heads + h) * D + lane * E;
 #pragma unroll
         for (int e = 0; e < E; e += 2) *reinterpret_cast<uint32_t*>(dst + e) = pack_bf16x2(acc[e] * inv, acc[e + 1] * inv);
@@ -844,7 +844,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) paged_join_many_kernel(const 
       }
 #pragma unroll
       for (int o = K / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      const float inv = sum > 0.f ? 1.f / sum : 0.f;
+      const float inv = 1.f / sum;
 #pragma unroll
       for (int j = 0; j < R; ++j) {
         const int r = r0 + j;
@@ -1210,7 +1210,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
         wait(&pv_done[x], ph ^ 1u);
         tc_fence_after();
         if (__any_sync(0xffffffffu, *abort_flag != 0)) break;
-        const float inv = l > 0.f ? 1.f / l : 0.f;
+        const float inv = 1.f / l;
 #pragma unroll
         for (int c0 = 0; c0 < D; c0 += 64) {  // all loads of 64 columns first: they take as long as one
           float v[2][2][16];

@@ -240,6 +240,30 @@ def test_attention_of_large_and_small_scores(device, new, wide):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("new", [1, 90])
+@pytest.mark.parametrize("wide", [3, 5000])
+def test_attention_of_no_numbers(device, new, wide):
+    """A query that is no number, and keys whose scores are all minus infinity, have no result that is a number, and the rows beside
+    them theirs."""
+    c = Paged([(700, new), (30, new)], 4, 2, 64, 16, device, wide=wide).fill()
+    q = torch.randn(c.tokens, 4, 64, device=device).bfloat16()
+    page, row = c.slots(0, 0, 700 + new)
+    c.k[page, row, 0, 3] = -math.inf
+    q[:new, :2, 3] = 1.0
+    q[new - 1, 3, 7] = math.nan
+    q[new, 1, 60] = math.nan
+    want, weight, big = _attend(q, c)
+    assert want[:new, :2].isnan().all() and want[new - 1, 3].isnan().all() and int(want.isnan().sum()) == (2 * new + 2) * 64
+    got = ops.paged_attention(q, *c.where())
+    if device == "cuda":
+        ops.check_status()
+    assert torch.equal(got.isnan(), want.isnan())
+    there = ~want.isnan()
+    bound = HALF_STEP * (weight + want.abs()) + weight * (4 * c.dim * 2 * U32 * big + 2.0 ** -16)  # as in _check_attention
+    assert ((got.double() - want).abs()[there] <= (bound * (1 + 2 ** -6) + 1e-38)[there]).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_attention_takes_scale_and_strided_queries(device):
     c = Paged([(50, 3), (0, 200)], 4, 4, 64, 16, device).fill()
     wide = torch.randn(c.tokens, 8, 64, device=device).bfloat16()
