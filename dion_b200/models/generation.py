@@ -8,12 +8,13 @@ the step asks for.  Both models of this package do.
 from __future__ import annotations
 
 from dataclasses import dataclass
-from typing import List, Optional, Sequence, Tuple
+from typing import Dict, List, Optional, Sequence, Tuple
 
 import torch
 import torch.nn.functional as F
 
 from ..ops import paged_append, paged_attention, verify_drafts
+from ..ops.nn import rotary_tables
 
 
 class PagedCache:
@@ -36,6 +37,7 @@ class PagedCache:
         self._pages: List[List[int]] = [[] for _ in range(sequences)]
         self._table = torch.zeros(sequences, each, dtype=torch.int32)
         self._on_device: Optional[torch.Tensor] = None
+        self._rotary: Dict[float, Tuple[torch.Tensor, torch.Tensor]] = {}
 
     @property
     def device(self) -> torch.device:
@@ -44,6 +46,13 @@ class PagedCache:
     @property
     def free_pages(self) -> int:
         return len(self._free)
+
+    def rotary(self, base: float) -> Tuple[torch.Tensor, torch.Tensor]:
+        """cos and sin of every position, for all layers.  The layers' own tables are left alone: a captured graph of theirs may
+        go on reading them."""
+        if base not in self._rotary:
+            self._rotary[base] = rotary_tables(self.max_len, self.k[0].shape[-1], self.device, base)
+        return self._rotary[base]
 
     def step(self, counts: Sequence[int], all_rows: bool = False) -> "CacheStep":
         """Room for ``counts[b]`` new tokens of each sequence (none is allowed), which count as cached from now on."""

@@ -114,7 +114,7 @@ class CausalSelfAttention(nn.Module):
         """The same for the new tokens of a cache's sequences, [1, tokens, C]."""
         q, k, v = (t.view(h.shape[1], -1, self.head_dim) for t in K.linear_fanout(
             h, _local(self.c_q.weight), _local(self.c_k.weight), _local(self.c_v.weight)))
-        y = step.attend(layer, q, k, v, *self.rotary.tables(step.cache.max_len, h.device), norm_eps=K.RMS_EPS)
+        y = step.attend(layer, q, k, v, *step.cache.rotary(self.rotary.base), norm_eps=K.RMS_EPS)
         return K.linear(y.view(1, h.shape[1], -1), _local(self.c_proj.weight), residual=residual)
 
 

@@ -82,7 +82,7 @@ class LlamaAttention(nn.Module):
     def forward_cached(self, h: torch.Tensor, residual: torch.Tensor, step: CacheStep, layer: int) -> torch.Tensor:
         """The same for the new tokens of a cache's sequences, [1, tokens, C]."""
         q, k, v = (K.linear(h, w.weight).view(h.shape[1], -1, self.head_dim) for w in (self.wq, self.wk, self.wv))
-        y = step.attend(layer, q, k, v, *self._rope(step.cache.max_len, h.device))
+        y = step.attend(layer, q, k, v, *step.cache.rotary(self.rope_theta))
         return K.linear(y.view(1, h.shape[1], -1), self.wo.weight, residual=residual)
 
 

@@ -117,6 +117,18 @@ def test_cached_passes_on_the_kernels(make, kw):
         assert ops.launch_count() > launches and done == [400, 400, 400]
 
 
+@pytest.mark.parametrize("make,tables", [(_gpt, lambda m: [x for b in m.transformer.h for x in (b.attn.rotary.cos_cached, b.attn.rotary.sin_cached)]),
+                                         (_llama, lambda m: [x for b in m.layers for x in b.attention._tables])])
+def test_the_layers_keep_their_rotation_tables(make, tables):
+    """What a captured pass of the model reads is still there after a cache has been used."""
+    m = make()
+    with torch.no_grad():
+        _whole_logits(m, torch.randint(0, 97, (2, 24)))
+        before = tables(m)
+        m(torch.randint(0, 97, (9,)), cache=m.new_cache(2).step([4, 5]))
+    assert all(a is b for a, b in zip(before, tables(m)))
+
+
 # --------------------------------------------------------------------------- sampling
 
 def test_cached_sampling_draws_the_same_tokens():
