@@ -55,9 +55,9 @@ class PagedCache:
         return self._rotary[base]
 
     def step(self, counts: Sequence[int], all_rows: bool = False) -> "CacheStep":
-        """Room for ``counts[b]`` new tokens of each sequence (none is allowed), which count as cached from now on."""
-        if len(counts) != len(self.lengths) or any(n < 0 for n in counts):
-            raise ValueError(f"{len(self.lengths)} sequences need as many counts, none below zero, not {list(counts)}")
+        """Room for ``counts[b]`` new tokens of each sequence (none is allowed, not of all), which count as cached from now on."""
+        if len(counts) != len(self.lengths) or any(n < 0 for n in counts) or not any(counts):
+            raise ValueError(f"{len(self.lengths)} sequences need as many counts, none below zero, one above, not {list(counts)}")
         ends = [p + n for p, n in zip(self.lengths, counts)]
         if max(ends) > self.max_len:
             raise ValueError(f"a sequence of {max(ends)} tokens in a cache for {self.max_len}")
@@ -76,7 +76,7 @@ class PagedCache:
             offsets.append(offsets[-1] + n)
         past, self.lengths = self.lengths, ends
         small = torch.tensor([offsets, past + [0]], dtype=torch.int32).to(self.device)
-        return CacheStep(self, self._on_device, small[0], small[1, :-1], max(max(counts), 1),
+        return CacheStep(self, self._on_device, small[0], small[1, :-1], offsets[-1], max(counts),
                          None if all_rows else [e - 1 for e, n in zip(offsets[1:], counts) if n])
 
     def cut(self, lengths: Sequence[int]) -> None:
@@ -91,14 +91,23 @@ class PagedCache:
 
 @dataclass
 class CacheStep:
-    """One forward pass over a cache: which tokens are new, and of which rows the logits are wanted (None: of all)."""
+    """One forward pass over a cache: whose tokens are new, how many in all and of a sequence at most, and of which rows the
+    logits are wanted (None: of all)."""
 
     cache: PagedCache
     page_table: torch.Tensor
     offsets: torch.Tensor
     lengths: torch.Tensor
+    tokens: int
     max_new: int
     rows: Optional[List[int]]
+
+    def check(self, tokens: torch.Tensor, targets: Optional[torch.Tensor]) -> None:
+        """Refuses what a model's pass over this step cannot take."""
+        if targets is not None:
+            raise ValueError("a pass over a cache has no loss: targets go without")
+        if list(tokens.shape) != [self.tokens]:
+            raise ValueError(f"the step has room for {self.tokens} new tokens in one row, not for {list(tokens.shape)}")
 
     def attend(self, layer: int, q, k, v, cos, sin, norm_eps: Optional[float] = None) -> torch.Tensor:
         """Rotates, caches and attends: q, k, v of the new tokens, [tokens, heads, head_dim], to the attention's result."""
@@ -183,7 +192,7 @@ def generate_drafted(model, limit: int, draft_model, draft_limit: int, draft_tok
             step = drafts.step(counts(lambda b: have[b] - drafts.lengths[b]) if i == 0 else counts(lambda b: 1))
             q.append(probabilities(draft_model(feed, cache=step), temperature, top_k))
             proposed.append(torch.multinomial(q[-1], num_samples=1))
-        tokens = torch.cat(proposed, 1) if k else idx.new_zeros(len(active), 0)
+        tokens = torch.cat(proposed, 1) if k else torch.zeros(len(active), 0, dtype=torch.int64, device=device)
         last = idx[at, torch.tensor([have[b] - 1 for b in active], device=device)]
         logits = model(torch.cat([last[:, None], tokens], 1).reshape(-1), cache=cache.step(counts(lambda b: k + 1), all_rows=True))
         p = probabilities(logits, temperature, top_k).view(len(active), k + 1, -1)

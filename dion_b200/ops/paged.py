@@ -14,7 +14,8 @@ nobody: their results are zero, nothing of theirs is written to the pages.  Tabl
 As for the other model ops, bf16 tensors on a GPU (head dimension 64 or 128) run the kernels, anything else plain PyTorch of the
 same semantics.  The kernels never wait for the host and can be captured: what the host cannot see (a position beyond the page table
 or the rotation tables, a page that does not exist, offsets that run backwards) sets the device's status word, which
-``check_status`` raises, and touches no memory; the plain path raises ``ValueError``.  None of the three has a gradient: inputs that
+``check_status`` raises, and reaches no memory outside the tensors; the results of such a call are not to be used.  The plain path
+raises ``ValueError``.  None of the three has a gradient: inputs that
 ask for one are refused.
 """
 

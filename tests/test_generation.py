@@ -129,6 +129,33 @@ def test_the_layers_keep_their_rotation_tables(make, tables):
     assert all(a is b for a, b in zip(before, tables(m)))
 
 
+@pytest.mark.parametrize("make", [_gpt, _llama])
+def test_a_pass_over_a_cache_refuses_what_its_step_has_no_room_for(make):
+    m = make()
+    cache = m.new_cache(2)
+    with pytest.raises(ValueError, match="counts"):
+        cache.step([0, 0])
+    with torch.no_grad():
+        step = cache.step([3, 1])
+        for tokens in (torch.zeros(3, dtype=torch.long), torch.zeros(2, 2, dtype=torch.long)):
+            with pytest.raises(ValueError, match="room for 4"):
+                m(tokens, cache=step)
+        with pytest.raises(ValueError, match="targets"):
+            m(torch.zeros(4, dtype=torch.long), torch.zeros(4, dtype=torch.long), cache=step)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        m(torch.zeros(4, dtype=torch.long), cache=step)
+
+
+@pytest.mark.parametrize("new", [1, 2, 6])
+def test_prompts_of_32_bits_draw_the_same_tokens(new):
+    torch.manual_seed(10)
+    m = _gpt()
+    idx = torch.randint(0, 97, (3, 5))
+    want = m.generate(idx, new, top_k=1, use_cache=True)
+    assert torch.equal(m.generate(idx.int(), new, top_k=1, use_cache=True), want)
+    assert torch.equal(m.generate(idx.int(), new, top_k=1, draft_model=m, draft_tokens=2), want.int())
+
+
 # --------------------------------------------------------------------------- sampling
 
 def test_cached_sampling_draws_the_same_tokens():
