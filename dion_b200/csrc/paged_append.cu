@@ -110,7 +110,7 @@ __global__ void __launch_bounds__(kAppendThreads, T == 1 ? 1 : 6) paged_append_k
     if (T > 1 && t0 + j >= p.tokens) break;
     const long long at = of_k ? k_at[j] : v_at[j];
     uint4 a = lo[j], b = hi[j];
-    if (of_q || of_k) {
+    if ((of_q || of_k) && at >= 0) {  // nobody's row has no position, and the tables may not have a row either
       f32x2 x1[4], x2[4], c[4], s[4];
       unpack8(a, x1);
       unpack8(b, x2);

@@ -562,6 +562,29 @@ def test_positions_beyond_the_rotation_tables_are_reported(device):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dim,eps,wide", [(64, None, False), (64, 1e-6, True), (128, 1e-6, False), (128, None, True)])
+@pytest.mark.parametrize("new,tail", [(2, 0), (0, 3), (700, 5)])
+def test_rotation_tables_without_a_row(device, dim, eps, wide, new, tail):
+    """Every position lies beyond them, and rows that are nobody's need none: nothing is read from them and nothing is written
+    to the pages."""
+    c = Paged([(20, new), (5, 0)], 2, 2, dim, 16, device, garbage=7.0, tail=tail).fill()
+    q = torch.randn(c.tokens, 2, dim, device=device).bfloat16()
+    cos, sin = (t[:0].float() if wide else t[:0] for t in N.rotary_tables(8, dim, device))
+    was_k, was_v = c.k.clone(), c.v.clone()
+    if device == "cpu" and new:
+        with pytest.raises(ValueError, match="rotation tables"):
+            ops.paged_append(q, q, q, cos, sin, *c.where(), norm_eps=eps)
+        return
+    out = ops.paged_append(q, q, q, cos, sin, *c.where(), norm_eps=eps)
+    if new:
+        with pytest.raises(ops.DionKernelError, match="bad kernel argument"):
+            ops.check_status()
+    elif device == "cuda":
+        ops.check_status()
+    assert (out == 0).all() and torch.equal(c.k, was_k) and torch.equal(c.v, was_v)
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_more_new_tokens_than_announced(device):
     c = Paged([(20, 1), (5, 100)], 2, 2, 64, 16, device).fill()
     q = torch.randn(101, 2, 64, device=device).bfloat16()
