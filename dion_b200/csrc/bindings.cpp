@@ -1376,7 +1376,7 @@ Tensor with_rows(const Tensor& t) {
 std::optional<Tensor> paged_append(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& cos_, const Tensor& sin_, Tensor k_pages,
                     Tensor v_pages, const Tensor& page_table, const Tensor& offsets, const Tensor& lengths, double eps,
                     Tensor status) {
-  refuse_gradients("paged_append", {&q_, &k_, &v_, &k_pages, &v_pages});
+  refuse_gradients("paged_append", {&q_, &k_, &v_, &cos_, &sin_, &k_pages, &v_pages});
   if (!paged_on_kernels(q_)) return std::nullopt;
   TORCH_CHECK_VALUE(!(eps < 0.) || eps == -1., "paged_append: norm_eps is None or not negative, not ", eps);
   dion::PagedAppend p;

@@ -171,7 +171,7 @@ def paged_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.T
                                         -1.0 if norm_eps is None else norm_eps, runtime.status_tensor(q.device))
         if out is not None:
             return out
-    _no_gradients("paged_append", q, k, v, k_pages, v_pages)
+    _no_gradients("paged_append", q, k, v, cos, sin, k_pages, v_pages)
     return _append_plain(q, k, v, cos, sin, k_pages, v_pages, page_table, new_offsets, lengths, norm_eps)
 
 

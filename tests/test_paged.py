@@ -496,6 +496,21 @@ def test_gradients_are_refused(device):
             call()
 
 
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("which", ["cos", "sin"])
+def test_gradients_of_the_rotation_tables_are_refused(device, which):
+    c = Paged([(20, 2)], 2, 2, 64, 16, device, garbage=7.0).fill()
+    q = torch.randn(2, 2, 64, device=device).bfloat16()
+    tables = dict(zip(("cos", "sin"), N.rotary_tables(64, 64, device)))
+    tables[which] = tables[which].clone().requires_grad_()
+    was = c.both.clone()
+    with pytest.raises(RuntimeError, match="gradient"):
+        ops.paged_append(q, q, q, *tables.values(), *c.where())
+    assert torch.equal(c.both, was)
+    with torch.no_grad():
+        assert not ops.paged_append(q, q, q, *tables.values(), *c.where()).requires_grad
+
+
 def _bad(device):
     """(what, changed tensors) that only the values tell from good ones."""
     def table(c, b, i, to):
