@@ -2,6 +2,7 @@
 // torch.ops.dion_b200.* by loading the shared library; no Python C-API use.
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/library.h>
 #include <torch/torch.h>
@@ -1304,6 +1305,12 @@ void refuse_gradients(const char* name, std::initializer_list<const Tensor*> ten
   for (const Tensor* t : tensors)
     TORCH_CHECK(!t->defined() || !t->requires_grad(), name, " has no gradient: call it under torch.no_grad() or with detached inputs");
 }
+// Nor do the kernels carry forward-mode tangents, which no_grad leaves on.
+void refuse_tangents(const char* name, std::initializer_list<const Tensor*> tensors) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  for (const Tensor* t : tensors)
+    TORCH_CHECK(!t->defined() || !t->_fw_grad(0).defined(), name, " has no forward-mode derivative on the kernels: call it with plain tensors");
+}
 // Types and head dimensions that the kernels take; others go the plain way.
 bool paged_on_kernels(const Tensor& q) {
   return q.scalar_type() == at::kBFloat16 && q.dim() > 0 && (q.size(-1) == 64 || q.size(-1) == 128);
@@ -1378,6 +1385,7 @@ std::optional<Tensor> paged_append(const Tensor& q_, const Tensor& k_, const Ten
                     Tensor status) {
   refuse_gradients("paged_append", {&q_, &k_, &v_, &cos_, &sin_, &k_pages, &v_pages});
   if (!paged_on_kernels(q_)) return std::nullopt;
+  refuse_tangents("paged_append", {&q_, &k_, &v_, &cos_, &sin_, &k_pages, &v_pages});
   TORCH_CHECK_VALUE(!(eps < 0.) || eps == -1., "paged_append: norm_eps is None or not negative, not ", eps);
   dion::PagedAppend p;
   const c10::cuda::CUDAGuard guard(q_.device());
@@ -1413,6 +1421,7 @@ std::optional<Tensor> paged_attention(const Tensor& q_, const Tensor& k_pages, c
                        const Tensor& offsets, const Tensor& lengths, double scale, int64_t max_new, Tensor status) {
   refuse_gradients("paged_attention", {&q_, &k_pages, &v_pages});
   if (!paged_on_kernels(q_)) return std::nullopt;
+  refuse_tangents("paged_attention", {&q_, &k_pages, &v_pages});
   dion::PagedAttention p;
   const c10::cuda::CUDAGuard guard(q_.device());
   describe_paged(p, "paged_attention", q_, k_pages, v_pages, page_table, offsets, lengths, status);
@@ -1437,8 +1446,9 @@ std::optional<Tensor> paged_attention(const Tensor& q_, const Tensor& k_pages, c
 
 std::tuple<Tensor, Tensor> verify_drafts(const Tensor& target, const std::optional<Tensor>& draft, const Tensor& tokens,
                                          const Tensor& uniforms, Tensor status) {
-  refuse_gradients("verify_drafts", {&target, &uniforms});
-  if (draft.has_value()) refuse_gradients("verify_drafts", {&*draft});
+  const Tensor drawn_from = draft.value_or(Tensor());
+  refuse_gradients("verify_drafts", {&target, &drawn_from, &uniforms});
+  refuse_tangents("verify_drafts", {&target, &drawn_from, &uniforms});
   const c10::cuda::CUDAGuard guard(target.device());
   TORCH_CHECK_VALUE(target.dim() == 3 && target.size(1) >= 1 && target.size(2) >= 1 && target.scalar_type() == at::kFloat,
                     "verify_drafts: the target's probabilities are fp32 [sequences, drafts + 1, vocabulary], not ", target.scalar_type(), " ", target.sizes());

@@ -16,7 +16,7 @@ same semantics.  The kernels never wait for the host and can be captured: what t
 or the rotation tables, a page that does not exist, offsets that run backwards) sets the device's status word, which
 ``check_status`` raises, and reaches no memory outside the tensors; the results of such a call are not to be used.  The plain path
 raises ``ValueError``.  None of the three has a gradient: inputs that
-ask for one are refused.
+ask for one are refused, and the kernels refuse forward-mode tangents, which the plain path carries.
 """
 
 from __future__ import annotations

@@ -4,6 +4,7 @@ import math
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwd
 
 from dion_b200 import ops
 from dion_b200.ops import nn as N
@@ -509,6 +510,42 @@ def test_gradients_of_the_rotation_tables_are_refused(device, which):
     assert torch.equal(c.both, was)
     with torch.no_grad():
         assert not ops.paged_append(q, q, q, *tables.values(), *c.where()).requires_grad
+
+
+@pytest.mark.gpu
+def test_tangents_are_refused_by_the_kernels():
+    """A forward-mode derivative would be lost there, whichever input it comes with, and under no_grad too."""
+    c = Paged([(20, 2)], 2, 2, 64, 16, "cuda", garbage=7.0).fill()
+    q = torch.randn(2, 2, 64, device="cuda").bfloat16()
+    p, d = torch.rand(1, 2, 9, device="cuda"), torch.rand(1, 1, 9, device="cuda")
+    t, u = torch.zeros(1, 1, dtype=torch.long, device="cuda"), torch.rand(1, 2, device="cuda")
+    calls = [(lambda q, k, v, cos, sin, k_pages, v_pages: ops.paged_append(q, k, v, cos, sin, k_pages, v_pages, *c.where()[2:]),
+              (q, q, q, *N.rotary_tables(64, 64, "cuda"), c.k, c.v)),
+             (lambda q, k_pages, v_pages: ops.paged_attention(q, k_pages, v_pages, *c.where()[2:]), (q, c.k, c.v)),
+             (lambda p, d, u: ops.verify_drafts(p, d, t, u), (p, d, u))]
+    was = c.both.clone()
+    for call, args in calls:
+        for i, x in enumerate(args):
+            with fwd.dual_level():
+                dual = list(args)
+                dual[i] = fwd.make_dual(x, torch.ones_like(x))
+                for grad in (True, False):
+                    with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="forward-mode"):
+                        call(*dual)
+    assert torch.equal(c.both, was)
+    for call, args in calls:
+        call(*args)
+    ops.check_status()
+
+
+def test_the_plain_path_carries_tangents():
+    c = Paged([(20, 2)], 2, 2, 16, 16, "cpu", dtype=torch.float64).fill()
+    q, t = torch.randn(2, 2, 2, 16, dtype=torch.float64)
+    with fwd.dual_level():
+        got = fwd.unpack_dual(ops.paged_attention(fwd.make_dual(q, t), *c.where())).tangent
+    h = 1e-6  # the difference is off by h^2 / 6 of a third derivative, at most some tens here, and by roundings over 2 h
+    want = (ops.paged_attention(q + h * t, *c.where()) - ops.paged_attention(q - h * t, *c.where())) / (2 * h)
+    torch.testing.assert_close(got, want, rtol=0, atol=1e-7)
 
 
 def _bad(device):
