@@ -7,8 +7,9 @@ the step asks for.  Both models of this package do.
 
 from __future__ import annotations
 
+from contextlib import contextmanager
 from dataclasses import dataclass
-from typing import Dict, List, Optional, Sequence, Tuple
+from typing import Dict, Iterator, List, Optional, Sequence, Tuple
 
 import torch
 import torch.nn.functional as F
@@ -37,6 +38,7 @@ class PagedCache:
         self._pages: List[List[int]] = [[] for _ in range(sequences)]
         self._table = torch.zeros(sequences, each, dtype=torch.int32)
         self._on_device: Optional[torch.Tensor] = None
+        self._changes = 0  # of the lengths so far
         self._rotary: Dict[float, Tuple[torch.Tensor, torch.Tensor]] = {}
 
     @property
@@ -55,13 +57,14 @@ class PagedCache:
         return self._rotary[base]
 
     def step(self, counts: Sequence[int], all_rows: bool = False) -> "CacheStep":
-        """Room for ``counts[b]`` new tokens of each sequence (none is allowed, not of all), which count as cached from now on."""
+        """Room for ``counts[b]`` new tokens of each sequence (none is allowed, not of all), which count as cached from now on, unless
+        the model's pass over the step fails."""
         if len(counts) != len(self.lengths) or any(n < 0 for n in counts) or not any(counts):
             raise ValueError(f"{len(self.lengths)} sequences need as many counts, none below zero, one above, not {list(counts)}")
         ends = [p + n for p, n in zip(self.lengths, counts)]
         if max(ends) > self.max_len:
             raise ValueError(f"a sequence of {max(ends)} tokens in a cache for {self.max_len}")
-        need = [-(-e // self.page_size) - len(p) if n else 0 for e, n, p in zip(ends, counts, self._pages)]
+        need = [max(-(-e // self.page_size) - len(p), 0) if n else 0 for e, n, p in zip(ends, counts, self._pages)]
         if sum(need) > len(self._free):
             raise RuntimeError(f"the cache has {len(self._free)} free pages of {self.page_size} tokens, {sum(need)} are needed")
         for b, n in enumerate(need):
@@ -74,16 +77,18 @@ class PagedCache:
         offsets = [0]
         for n in counts:
             offsets.append(offsets[-1] + n)
+        small = torch.tensor([offsets, self.lengths + [0]], dtype=torch.int32).to(self.device)
         past, self.lengths = self.lengths, ends
-        small = torch.tensor([offsets, past + [0]], dtype=torch.int32).to(self.device)
+        self._changes += 1
         return CacheStep(self, self._on_device, small[0], small[1, :-1], offsets[-1], max(counts),
-                         None if all_rows else [e - 1 for e, n in zip(offsets[1:], counts) if n])
+                         None if all_rows else [e - 1 for e, n in zip(offsets[1:], counts) if n], list(counts), past, self._changes)
 
     def cut(self, lengths: Sequence[int]) -> None:
         """Shortens the sequences to `lengths`; pages that hold nothing any more go back to the pool."""
         if len(lengths) != len(self.lengths) or any(not 0 <= n <= p for n, p in zip(lengths, self.lengths)):
             raise ValueError(f"sequences of {self.lengths} tokens cannot be cut to {list(lengths)}")
         self.lengths = list(lengths)
+        self._changes += 1
         for pages, n in zip(self._pages, lengths):
             while len(pages) > -(-n // self.page_size):
                 self._free.append(pages.pop())
@@ -101,6 +106,31 @@ class CacheStep:
     tokens: int
     max_new: int
     rows: Optional[List[int]]
+    counts: Sequence[int] = ()  # of each sequence: its new tokens, and those that were cached before
+    past: Sequence[int] = ()
+    change: int = -1  # which of the cache's changes this step was
+    state: str = "taken"  # or "passed", or "back" where the cache has taken the tokens back
+
+    @contextmanager
+    def passing(self, tokens: torch.Tensor, targets: Optional[torch.Tensor]) -> Iterator[None]:
+        """Around a model's pass over this step.  Where the pass fails, the pages may hold anything in place of its tokens: if nothing
+        has changed the lengths since, the cache is then as it was before the step, which can be passed again or dropped."""
+        try:
+            self.check(tokens, targets)
+            if self.state == "back":
+                if self.cache.lengths != list(self.past):
+                    raise ValueError("a pass over this step has failed and the cache has changed since: take another step")
+                again = self.cache.step(self.counts)
+                self.page_table, self.offsets, self.lengths, self.change = again.page_table, again.offsets, again.lengths, again.change
+            self.state = "taken"
+            yield
+            self.state = "passed"
+        except BaseException:
+            ends = [p + n for p, n in zip(self.past, self.counts)]
+            if self.state == "taken" and self.cache._changes == self.change and self.cache.lengths == ends:
+                self.cache.cut(self.past)
+                self.state = "back"
+            raise
 
     def check(self, tokens: torch.Tensor, targets: Optional[torch.Tensor]) -> None:
         """Refuses what a model's pass over this step cannot take."""

@@ -234,8 +234,8 @@ class GPT(nn.Module):
     # -- forward
     def forward(self, idx, targets=None, return_logits=False, cache: Optional[CacheStep] = None):
         if cache is not None:
-            cache.check(idx, targets)
-            return self._forward_cached(idx, cache)
+            with cache.passing(idx, targets):
+                return self._forward_cached(idx, cache)
         bt = self._sequence_parallel_shape(idx)
         x = self._forward_emb(idx, bt)
         return self._forward(x, targets, return_logits, bt)

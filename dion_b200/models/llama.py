@@ -137,8 +137,8 @@ class Llama(nn.Module):
     def forward(self, idx: torch.Tensor, targets: Optional[torch.Tensor] = None, return_logits: bool = False,
                 cache: Optional[CacheStep] = None):
         if cache is not None:
-            cache.check(idx, targets)
-            return self._forward_cached(idx, cache)
+            with cache.passing(idx, targets):
+                return self._forward_cached(idx, cache)
         dtype = torch.bfloat16 if idx.is_cuda else self.output.weight.dtype
         x = K.embedding(idx, self.tok_embeddings.weight, dtype)
         for layer in self.layers:

@@ -146,6 +146,69 @@ def test_a_pass_over_a_cache_refuses_what_its_step_has_no_room_for(make):
         m(torch.zeros(4, dtype=torch.long), cache=step)
 
 
+@pytest.mark.parametrize("make", [_gpt, _llama])
+def test_a_pass_that_fails_leaves_the_cache_as_it_was(make):
+    """Wrong tokens, gradients left on, a layer that raises half way: the tokens count as cached no longer, and another step, or the
+    same one again, gives the logits of a cache that has seen no failure."""
+    torch.manual_seed(11)
+    m = make()
+    tokens = torch.randint(0, 97, (22,))
+    first, then = tokens[:20], torch.cat([tokens[20:], tokens[:1]])
+    with torch.no_grad():
+        good = m.new_cache(2, page_size=16)
+        m(first, cache=good.step([14, 6]))
+        want = m(then, cache=good.step([3, 0], all_rows=True))
+
+    def broken(*_):
+        raise KeyError("half way")
+
+    layers = m.transformer.h if make is _gpt else m.layers
+    for again in (False, True):
+        cache = m.new_cache(2, page_size=16)
+        with torch.no_grad():
+            m(first, cache=cache.step([14, 6]))
+        free = cache.free_pages
+        step = cache.step([3, 0], all_rows=True)
+        assert cache.lengths == [17, 6] and cache.free_pages == free - 1
+        with pytest.raises(RuntimeError, match="no gradient"):
+            m(then, cache=step)
+        assert cache.lengths == [14, 6] and cache.free_pages == free
+        with torch.no_grad():
+            with pytest.raises(ValueError, match="room for"):
+                m(then[:2], cache=step if again else cache.step([3, 0], all_rows=True))
+            assert cache.lengths == [14, 6] and cache.free_pages == free
+            hook = layers[1].register_forward_pre_hook(broken)
+            with pytest.raises(KeyError):
+                m(tokens[:3], cache=step if again else cache.step([3, 0]))
+            hook.remove()
+            assert cache.lengths == [14, 6] and cache.free_pages == free
+            got = m(then, cache=step if again else cache.step([3, 0], all_rows=True))
+            assert cache.lengths == [17, 6] and torch.equal(got, want)
+            with pytest.raises(ValueError, match="room for"):  # what a pass has cached stays
+                m(then[:2], cache=step)
+            assert cache.lengths == [17, 6]
+
+
+@pytest.mark.parametrize("make", [_gpt, _llama])
+def test_a_failed_step_does_not_take_back_what_came_after(make):
+    m = make()
+    cache = m.new_cache(2, page_size=16)
+    with torch.no_grad():
+        one = cache.step([3, 1])
+        m(torch.zeros(5, dtype=torch.long), cache=cache.step([0, 5]))
+        with pytest.raises(ValueError, match="room for"):
+            m(torch.zeros(5, dtype=torch.long), cache=one)
+        assert cache.lengths == [3, 6]
+        cache.cut([0, 0])
+        one = cache.step([3, 1])
+        with pytest.raises(ValueError, match="room for"):
+            m(torch.zeros(5, dtype=torch.long), cache=one)
+        m(torch.zeros(5, dtype=torch.long), cache=cache.step([0, 5]))
+        with pytest.raises(ValueError, match="take another step"):
+            m(torch.zeros(4, dtype=torch.long), cache=one)
+        assert cache.lengths == [0, 5]
+
+
 @pytest.mark.parametrize("new", [1, 2, 6])
 def test_prompts_of_32_bits_draw_the_same_tokens(new):
     torch.manual_seed(10)
