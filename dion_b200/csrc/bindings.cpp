@@ -1399,6 +1399,7 @@ std::optional<Tensor> paged_append(const Tensor& q_, const Tensor& k_, const Ten
     TORCH_CHECK_VALUE(t->dim() == 2 && t->size(1) == D / 2 && t->sizes() == cos_.sizes() && t->scalar_type() == cos_.scalar_type() &&
                           (t->scalar_type() == at::kBFloat16 || t->scalar_type() == at::kFloat) && t->device() == q_.device(),
                       "paged_append: cos and sin are two tables [positions, ", D / 2, "] of one type, bf16 or fp32, on the device of the queries");
+  TORCH_CHECK_VALUE(cos_.size(0) <= std::numeric_limits<int>::max(), "paged_append: more than 2^31 - 1 rows of the rotation tables");
   if (N == 0 || p.seqs == 0) return at::zeros({N, p.heads, D}, q_.options());
   auto table = [](const Tensor& t) {
     return on_16_bytes(t) && t.stride(1) == 1 && t.stride(0) * t.element_size() % 16 == 0 ? t : t.clone(at::MemoryFormat::Contiguous);

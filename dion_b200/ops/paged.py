@@ -99,6 +99,8 @@ def _append_plain(q, k, v, cos, sin, k_pages, v_pages, page_table, new_offsets, 
     half = q.shape[2] // 2
     if q.shape[2] % 2 or cos.dim() != 2 or cos.shape[1] != half or sin.shape != cos.shape or sin.dtype != cos.dtype:
         raise ValueError(f"paged_append: cos and sin are two tables [positions, {half}] of one type")
+    if cos.shape[0] >= 2 ** 31:
+        raise ValueError("paged_append: more than 2^31 - 1 rows of the rotation tables")
     if any(n and p + n > cos.shape[0] for p, _, n in layout):
         raise ValueError(f"paged_append: a position beyond the {cos.shape[0]} rows of the rotation tables")
     out = torch.zeros(q.shape, dtype=q.dtype, device=q.device)

@@ -483,6 +483,21 @@ def test_refusals_of_shapes_and_types(device):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+def test_rotation_tables_beyond_32_bits_are_refused(device):
+    """Positions are 32-bit numbers in the kernel.  One row of either table, which stands for all of them, in no memory."""
+    c = Paged([(20, 2)], 2, 2, 64, 16, device).fill()
+    q = torch.randn(2, 2, 64, device=device).bfloat16()
+    cos, sin = (t[:1] for t in N.rotary_tables(1, 64, device))
+    for rows, good in ((2 ** 31 - 1, True), (2 ** 31, False)):
+        tables = cos.expand(rows, -1), sin.expand(rows, -1)
+        if good:
+            ops.paged_append(q, q, q, *tables, *c.where())
+        else:
+            with pytest.raises(ValueError, match="2\\^31"):
+                ops.paged_append(q, q, q, *tables, *c.where())
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_gradients_are_refused(device):
     c = Paged([(20, 2)], 2, 2, 64, 16, device).fill()
     q = torch.randn(2, 2, 64, device=device).bfloat16().requires_grad_()
