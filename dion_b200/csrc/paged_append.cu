@@ -154,8 +154,10 @@ cudaError_t append_launch(const PagedAppend& p, cudaStream_t stream) {
   const int parts = (rows + most - 1) / most, each = ((rows + parts - 1) / parts + step - 1) / step * step;  // blocks of a token, rows of one
   if (parts > 65535) return cudaErrorInvalidValue;
   const dim3 block(each * (HD / 16));
-  // one token a block while that leaves SMs without a block
-  if ((long long)p.tokens * parts <= 4ll * 148 * kAppendTokens)
+  // One token a block up to eight blocks per SM, where the shorter chain counts.  In a graph (us, one token / kAppendTokens): 6 + 2 x 6
+  // heads of 128, 64 tokens 2.4 / 2.9, 900 3.3 / 4.4, 1200 5.1 / 5.4, 2400 8.5 / 7.6; 32 + 2 x 8 (two blocks a token), 450 tokens
+  // 5.5 / 6.0, 600 6.8 / 6.5, 9600 51.4 / 44.4; 12 + 2 x 12 of 64, 900 3.3 / 4.3, 2400 8.5 / 7.2.
+  if ((long long)p.tokens * parts <= 8ll * attn_grid(1 << 20))
     return launch_pdl(paged_append_kernel<HD, 1, Table>, dim3(p.tokens, parts), block, 0, stream, 0, p);
   return launch_pdl(paged_append_kernel<HD, kAppendTokens, Table>, dim3((p.tokens + kAppendTokens - 1) / kAppendTokens, parts), block, 0, stream, 0, p);
 }
