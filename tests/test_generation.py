@@ -274,6 +274,43 @@ def test_drafted_sampling_runs_on_its_own_draws():
         m.generate(idx, 30, draft_model=_gpt(seq=32))
 
 
+@pytest.mark.parametrize("make,top_k", [(_gpt, None), (_llama, 3)])
+def test_drafted_sampling_is_distributed_as_without_a_draft(make, top_k):
+    """Three tokens of a vocabulary of five, temperature 0.7, from a draft of another opinion.  The counts of the 125 outcomes against the
+    products of the model's probabilities: the chi-square sum has its degrees of freedom as mean and twice these as variance, of
+    which four standard deviations are allowed.  Sequences finish after different numbers of passes.  What the draft, or the model at
+    another temperature, would say is far outside."""
+    torch.manual_seed(12)
+    m, small = make(vocab=5, seq=16), make(layers=1, width=32, heads=2, vocab=5, seq=16, **(dict(kv_heads=1) if make is _llama else {}))
+    with torch.no_grad():
+        for w in (*m.parameters(), *small.parameters()):
+            if w.dim() == 2:
+                w.normal_(std=2 * w.shape[1] ** -0.5)
+    n, new = 2000, 3
+    prompt = torch.tensor([[1, 4, 2]])
+    out = m.generate(prompt.expand(n, -1), new, temperature=0.7, top_k=top_k, draft_model=small, draft_tokens=2)
+    counts = torch.bincount(out[:, 3] * 25 + out[:, 4] * 5 + out[:, 5], minlength=125).double()
+
+    def outcomes(model, temperature=0.7):
+        every = torch.cartesian_prod(*[torch.arange(5)] * new)
+        with torch.no_grad():
+            logits = model(torch.cat([prompt.expand(125, -1), every], 1), torch.zeros(125, 3 + new, dtype=torch.long), return_logits=True).double()
+        logits = logits[:, 2:2 + new] / temperature
+        if top_k is not None:
+            logits = logits.masked_fill(logits < logits.topk(top_k).values[..., -1:], -torch.inf)
+        return torch.softmax(logits, -1).gather(-1, every[..., None]).prod(1)[:, 0]
+
+    def far(p):  # outcomes that are expected fewer than five times count as one
+        often = p * n >= 5
+        e, c = (torch.cat([t[often], t[~often].sum()[None]]) for t in (p * n, counts))
+        e, c = e[e > 0], c[e > 0]
+        return ((c - e).square() / e).sum().item() / (len(e) - 1 + 4 * (2 * (len(e) - 1)) ** 0.5)
+
+    p = outcomes(m)
+    assert abs(p.sum().item() - 1) < 1e-6 and (counts[p == 0] == 0).all()
+    assert far(p) <= 1 and far(outcomes(small).clamp_min(1e-9)) > 2 and far(outcomes(m, 1.0)) > 2
+
+
 @pytest.mark.gpu
 def test_generation_on_the_kernels():
     """Cached and drafted sampling through all operators.  With a draft that is the model itself nearly everything is accepted: fewer

@@ -359,6 +359,59 @@ def test_append_and_attention_in_a_graph_and_on_another_stream(new, wide):
     ops.check_status()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("new,wide", [(1, 8), (2, 5000), (90, 5000)])
+def test_a_graph_follows_the_pages_as_they_move(new, wide):
+    """Captured once; between replays the pages go to other places, the table is changed in place to match, sequences grow and the
+    inputs change.  Results and pages against the definitions, and rows that are nobody's as they were."""
+    c = Paged([(40, new), (300, new), (0, new)], 8, 4, 64, 16, "cuda", wide=wide, garbage=3.0, spare=9).fill(upto_new=False)
+    room = [int((row >= 0).sum()) * 16 for row in c.table]  # of each sequence's pages
+    cos, sin = N.rotary_tables(512, 64, "cuda")
+    qkv = torch.randn(c.tokens, 16, 64, device="cuda").bfloat16()
+
+    def call():
+        q, k, v = qkv.split([8, 4, 4], 1)
+        turned = ops.paged_append(q, k, v, cos, sin, *c.where(), norm_eps=1e-6)
+        return turned, ops.paged_attention(turned, *c.where(), max_new=new)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            turned, out = call()
+    torch.cuda.synchronize()
+    for step in range(4):
+        to = torch.randperm(c.k.shape[0], device="cuda")  # page i goes to to[i]
+        for t in (c.k, c.v):
+            moved = torch.empty_like(t)
+            moved[to] = t
+            t.copy_(moved)
+        c.table.copy_(torch.where(c.table >= 0, to[c.table.clamp_min(0).long()].int(), c.table))
+        c.sizes = [(max(0, min(p + (3 if step % 2 else -5), r - n)), n) for (p, n), r in zip(c.sizes, room)]
+        c.lengths.copy_(torch.tensor([p for p, _ in c.sizes], dtype=torch.int32))
+        qkv.copy_(torch.randn(qkv.shape, device="cuda"))
+        q, k, v = qkv.split([8, 4, 4], 1)
+        was_k, was_v = c.k.clone(), c.v.clone()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            g.replay()
+        torch.cuda.current_stream().wait_stream(side)
+        ops.check_status()
+        touched = torch.zeros(c.k.shape[:2], dtype=torch.bool, device="cuda")
+        for b, (p, n) in enumerate(c.sizes):
+            rows = slice(c.starts[b], c.starts[b] + n)
+            at = c.slots(b, p, p + n)
+            touched[at] = True
+            for got, x in ((turned[rows], q[rows]), (c.k[at], k[rows])):
+                want, most = _turned(x, cos[p:p + n], sin[p:p + n], 1e-6)
+                assert ((got.double() - want).abs() <= HALF_STEP * want.abs() + 2 * U32 * (8 + 64) * most + 1e-38).all()  # as in test_append
+            assert torch.equal(c.v[at], v[rows])
+        assert torch.equal(c.k[~touched], was_k[~touched]) and torch.equal(c.v[~touched], was_v[~touched])
+        _check_attention(out, turned, c)
+
+
 # --------------------------------------------------------------------------- check of drafts
 
 def _verify(p, q, tokens, u):
@@ -413,6 +466,30 @@ def test_verify_at_the_borders(device):
     p[4, 0, 1], p[4, 0, 4], q[4, 0, 1], q[4, 0, 4] = 0.25, 0.25, 0.5, 0.5  # nothing is left over: the target's row itself
     got = ops.verify_drafts(*(t.to(device) for t in (p, q, tokens, u)))
     assert got[0].tolist() == [1, 0, 0, 0, 0] and got[1].tolist() == [3, 6, 3, 0, 1]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("seqs,drafts,vocab,top_k", [(16, 4, 50304, 50), (24, 7, 128256, 50), (9, 3, 50304, 1), (5, 2, 128256, 3), (12, 5, 40001, 7)])
+@pytest.mark.parametrize("certain", [False, True])
+def test_verify_of_rows_that_are_mostly_zeros(device, seqs, drafts, vocab, top_k, certain):
+    """What sampling from the most likely tokens hands over: the distributions' few tokens anywhere, and partly the same ones."""
+    if device == "cpu":
+        seqs = min(seqs, 4)
+    logits = torch.randn(seqs, drafts + 1, vocab) * 2
+
+    def top(x):
+        return torch.softmax(x.masked_fill(x < x.topk(top_k).values[..., -1:], -math.inf), -1)
+
+    p, q = top(logits), None if certain else top(logits[:, :drafts] + torch.randn(seqs, drafts, vocab) * 0.1)
+    tokens = torch.multinomial((p[:, :drafts] if certain else q).reshape(-1, vocab), 1).view(seqs, drafts)
+    u = torch.rand(seqs, drafts + 1)
+    u[0], u[-1, -1] = 0.0, 1 - 2.0 ** -24
+    want = _verify(p, q, tokens, u)
+    got = ops.verify_drafts(*[None if t is None else t.to(device) for t in (p, q, tokens, u)])
+    if device == "cuda":
+        ops.check_status()
+    assert all(torch.equal(g.cpu(), w) for g, w in zip(got, want))
+    assert (p[torch.arange(seqs), want[0], want[1]] > 0).all()
 
 
 @pytest.mark.parametrize("device", DEVICES)
