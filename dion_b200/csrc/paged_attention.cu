@@ -1328,7 +1328,7 @@ struct Plan {
       // page table, which is all that the host knows: at most 4096 each, or 1024 where the clusters leave half of the SMs idle.  Both ways
       // (us, shares / clusters; 32 heads on 8 of 128): one token over 1000 keys 12.0 / 6.9, over 4000 13.7 / 9.0, over 16000 17.5 / 20.5;
       // 8 of 8000 52.0 / 44.7, 32 of up to 4000 54.2 / 48.2, 64 of 1000 54.7 / 46.0, 64 of 4000 165.7 / 149.5; of 8000 keys a CTA 40 items
-      // 201 / 227, 64 of up to 8000 138 / 131.
+      // 201 / 227, which the limit of 4096 is for, 64 of up to 8000, where clusters would be the better ones, 138 / 131.
       const long long most = (p.max_new + tl.per - 1) / tl.per, all = (long long)p.seqs * tl.heads * most;
       const long long slots = (long long)sms * (head_dim == 64 && tl.height < 64 ? 3 : 2);
       const long long likely = (long long)p.seqs * tl.heads * ((typical + tl.per - 1) / tl.per);

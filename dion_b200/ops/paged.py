@@ -184,7 +184,9 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     themselves: ``softmax(scale q K^T) V`` per head, ``[tokens, heads, head_dim]``.  `lengths` is what it was for ``paged_append``:
     without the new tokens.  Grouped heads: the kv heads divide the heads.  `scale` defaults to ``1 / sqrt(head_dim)``.  What lies in the
     pages behind a sequence's last token has no influence; the values of its own tokens meet every row of their chunk, those of later
-    ones with weight zero, and have to be finite.
+    ones with weight zero, and have to be finite.  The kernels round the softmax's weights to bf16 before they meet the values, their sum is
+    that of the unrounded ones in fp32: an output is off by at most a half step of bf16 of ``sum p |v|`` beside its own rounding.  The
+    plain path keeps fp32 weights.
 
     `max_new`: the most new tokens of a sequence, where the host knows it; a longer sequence is an error.  It goes into the choice
     of the kernel, as does the width of the page table, which says how long a sequence can be; any choice gives the result, to its
